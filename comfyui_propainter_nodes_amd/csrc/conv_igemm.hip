@@ -26,6 +26,7 @@ int convk_from_params(const pp_conv2d_params* p, ConvK* kp, const char* who, boo
   if (p->out_dtype != PP_F32 && p->out_dtype != PP_F16) return fail2(PP_ERR_UNSUPPORTED, who, "out_dtype");
   if (!p->weight || !p->out) return fail2(PP_ERR_BAD_ARG, who, "null weight/out");
   if (p->Z < 1 || p->Z > 65535) return fail2(PP_ERR_BAD_ARG, who, "Z out of range");
+  if (p->act == PP_ACT_SILU || p->act2 == PP_ACT_SILU) return fail2(PP_ERR_UNSUPPORTED, who, "PP_ACT_SILU is for pp_groupnorm");
   if (p->epi != PP_EPI_NONE && !p->aux1) return fail2(PP_ERR_BAD_ARG, who, "epilogue needs aux1");
   if (p->epi == PP_EPI_GRU && !p->aux2) return fail2(PP_ERR_BAD_ARG, who, "GRU epilogue needs aux2");
   // (r06: the PP_F32X2 patch form -- flat_taps on an f32 input of 1..4 channels, conv_patch.hip -- reads its input with 4-byte

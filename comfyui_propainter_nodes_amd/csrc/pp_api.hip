@@ -135,6 +135,9 @@ extern "C" int64_t pp_struct_size(const char* name) {
   PP_SIZEOF_CASE(pp_im2col_params)
   PP_SIZEOF_CASE(pp_split_pack_params)
   PP_SIZEOF_CASE(pp_instnorm_params)
+  PP_SIZEOF_CASE(pp_groupnorm_params)
+  PP_SIZEOF_CASE(pp_prompt_attention_params)
+  PP_SIZEOF_CASE(pp_prefix_attention_params)
   PP_SIZEOF_CASE(pp_avgpool2x2_params)
   PP_SIZEOF_CASE(pp_corr_lookup_params)
   PP_SIZEOF_CASE(pp_convex_upsample_params)

@@ -1,0 +1,211 @@
+// prefix_attention.hip -- attention of a batch whose sequences share a prefix and have own keys behind it.
+// Contract: include/propainter_mi355.h (pp_prefix_attention); the inner loop: tile_attention.h.
+//
+// All B L G rows of a key / value head (G = H / KH query heads share it) meet the same prefix keys: they are tiled 128 at a time, so a
+// prefix of P keys is staged ceil(B L G / 128) times instead of B times, and the two products run at matrix speed.  The prefix is
+// cut into pieces so that few rows still fill the chip; the own keys of a sequence (its L G rows) are work-groups of the same launch.  Every piece
+// leaves (maximum, sum, sum of weighted values) in fp32; a second launch joins them in piece order.
+#include "tile_attention.h"
+#include "pp_host.h"
+
+#include <math.h>
+
+namespace pp {
+
+struct PrefixK {
+  const void *q, *kp, *vp, *ko, *vo;
+  void* out;
+  const int* own_len;
+  float* part_o;   // [row][part][D]
+  float* part_ml;  // [row][part][2]
+  int64_t q_seq, q_row, q_head, kp_row, kp_head, vp_row, vp_head, ko_seq, ko_row, ko_head, vo_seq, vo_row, vo_head, out_seq, out_row, out_head;
+  int64_t P, S;
+  int B, L, H, KH, G, D, prefix_splits, own_splits, parts;
+  int prefix_tiles, own_tiles;  // 128-row tiles of all B L G rows / of one sequence's L G rows
+  int64_t prefix_items;         // work-groups of the prefix part; those of the own part follow
+  float sc;
+};
+
+constexpr int kRows = 128;
+
+template <typename Tile>
+__global__ void __launch_bounds__(256) prefix_attention_kernel(const PrefixK a) {
+  typedef typename Tile::type T;
+  const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
+  const bool shared = (int64_t)blockIdx.x < a.prefix_items;
+  int64_t id = shared ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - a.prefix_items;
+  const int kh = (int)(id % a.KH);
+  id /= a.KH;
+  const int lg = a.L * a.G;
+  int seq = 0, part;
+  int64_t row0, rows, n0, n1;  // rows of the item's tile space; its keys
+  const T *k, *v;
+  int64_t k_row, v_row, visible = 0;
+  if (shared) {
+    const int tile = (int)(id % a.prefix_tiles);
+    part = (int)(id / a.prefix_tiles);
+    rows = (int64_t)a.B * lg;
+    row0 = (int64_t)tile * kRows;
+    n0 = a.P * part / a.prefix_splits;
+    n1 = a.P * (part + 1) / a.prefix_splits;
+    k = (const T*)a.kp + kh * a.kp_head;
+    v = (const T*)a.vp + kh * a.vp_head;
+    k_row = a.kp_row;
+    v_row = a.vp_row;
+  } else {
+    const int tile = (int)(id % a.own_tiles);
+    id /= a.own_tiles;
+    const int sp = (int)(id % a.own_splits);
+    seq = (int)(id / a.own_splits);
+    part = a.prefix_splits + sp;
+    rows = lg;
+    row0 = (int64_t)tile * kRows;
+    const int64_t len = a.own_len[seq];
+    visible = len < 0 ? 0 : len > a.S ? a.S : len;
+    n0 = visible * sp / a.own_splits;
+    n1 = visible * (sp + 1) / a.own_splits;
+    k = (const T*)a.ko + seq * a.ko_seq + kh * a.ko_head;
+    v = (const T*)a.vo + seq * a.vo_seq + kh * a.vo_head;
+    k_row = a.ko_row;
+    v_row = a.vo_row;
+  }
+  // keys of [n0, n1) that a row sees
+  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int64_t {
+    if (shared) return n1 - n0;
+    const int64_t c = visible - a.L + row / a.G + 1 - n0;
+    return c < 0 ? 0 : c > n1 - n0 ? n1 - n0 : c;
+  };
+  const int64_t last = rows - 1;
+  const int64_t wrow = row0 + 32 * wave, row = wrow + q32;
+  const bool live = row <= last;
+  const int64_t limit = live ? limit_of(row) : 0;
+  const int64_t wave_min = wrow <= last ? limit_of(wrow) : 0;
+  const int64_t wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
+  const int64_t nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
+
+  const int64_t r = live ? row : 0;
+  const int64_t b = shared ? r / lg : seq;
+  const int in_seq = (int)(shared ? r % lg : r);
+  const int tok = in_seq / a.G, head = kh * a.G + in_seq % a.G;
+  Tile t;
+  AttnState<Tile> st;
+  t.init(PP_DYN_SMEM);
+  t.load_q(live ? (const T*)a.q + b * a.q_seq + tok * a.q_row + head * a.q_head : nullptr, a.D);
+  attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, nkeys, limit, wave_min, wave_max, a.D, a.sc);
+  if (!live) return;
+  const int64_t at = ((b * a.L + tok) * a.H + head) * a.parts + part;
+  float* dst = a.part_o + at * a.D;
+#pragma unroll
+  for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * db + 8 * g + 4 * h;
+      if (d < a.D) *reinterpret_cast<f4*>(dst + d) = f4{st.o[db][4 * g], st.o[db][4 * g + 1], st.o[db][4 * g + 2], st.o[db][4 * g + 3]};
+    }
+  if (h == 0) {
+    a.part_ml[2 * at] = st.m;
+    a.part_ml[2 * at + 1] = st.l;
+  }
+}
+
+// joins the parts of a row: one thread per 4 head-dim values
+template <typename Tile>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixK a) {
+  typedef typename Tile::type T;
+  const int per = a.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.L * a.H;
+  if (i >= rows * per) return;
+  const int64_t row = i / per;
+  const int d = (int)(i - row * per) * 4;
+  const float* ml = a.part_ml + row * a.parts * 2;
+  const float* po = a.part_o + row * a.parts * a.D + d;
+  float m = neg_inf();
+  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, ml[2 * p]);
+  float l = 0.f;
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < a.parts; ++p) {
+    const float mp = ml[2 * p];
+    const float w = mp == m ? 1.f : fast_exp2((mp - m) * a.sc);
+    l += w * ml[2 * p + 1];
+    o += w * *reinterpret_cast<const f4*>(po + (int64_t)p * a.D);
+  }
+  const int64_t bl = row / a.H, head = row - bl * a.H, b = bl / a.L, tok = bl - b * a.L;
+  // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
+  const int64_t own = a.own_len[b] > a.S ? a.S : a.own_len[b];
+  const float inv = a.P > 0 || own - a.L + tok + 1 > 0 ? 1.f / l : 0.f;
+  Tile::store4((T*)a.out + b * a.out_seq + tok * a.out_row + head * a.out_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+}
+
+}  // namespace pp
+
+template <typename T, int DP>
+static int launch_prefix(void* stream, const pp::PrefixK& a) {
+  using namespace pp;
+  typedef AttnTile<T, DP> Tile;
+  const int64_t items = a.prefix_items + (int64_t)a.own_splits * a.B * a.own_tiles * a.KH;
+  if (items * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the launch needs 2^32 threads or more");
+  PP_ALLOW_BIG_LDS((&prefix_attention_kernel<Tile>), Tile::kSmem);
+  if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(256), Tile::kSmem, stream, a);
+  const int rc = pp_check_launch("pp_prefix_attention");
+  if (rc != PP_OK) return rc;
+  PP_LAUNCH((prefix_join_kernel<Tile>), dim3(pp_blocks_1d((int64_t)a.B * a.L * a.H * (a.D / 4))), dim3(256), 0, stream, a);
+  return pp_check_launch("pp_prefix_attention(join)");
+}
+
+template <typename T>
+static int launch_prefix_d(void* stream, const pp::PrefixK& a) {
+  if (a.D <= 32) return launch_prefix<T, 32>(stream, a);
+  if (a.D <= 64) return launch_prefix<T, 64>(stream, a);
+  if (a.D <= 96) return launch_prefix<T, 96>(stream, a);
+  if (a.D <= 128) return launch_prefix<T, 128>(stream, a);
+  return launch_prefix<T, 256>(stream, a);
+}
+
+extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_params* p) {
+  using namespace pp;
+  if (!p || !p->q || !p->out || !p->own_len || !p->scratch) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: null argument");
+  if (p->dtype != PP_F32 && p->dtype != PP_F16 && p->dtype != PP_BF16) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: dtype");
+  if (p->KH < 1 || p->H < 1 || p->H % p->KH || p->H > (1 << 20))
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: H must be a multiple of KH");
+  const int e = p->dtype == PP_F32 ? 4 : 8;  // elements of 16 bytes
+  if (p->D < 1 || p->D > 256 || p->D % e) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: D must be a multiple of 8 (fp32: 4) up to 256");
+  if (p->B < 0 || p->L < 0 || p->P < 0 || p->S < 0 || p->B > (1 << 24) || p->L > (1 << 20) || p->P > INT32_MAX || p->S > INT32_MAX)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: B, L, P, S out of range");
+  if ((p->P > 0 && (!p->kp || !p->vp)) || (p->S > 0 && (!p->ko || !p->vo))) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: null keys or values");
+  if (p->prefix_splits < 0 || p->own_splits < 0 || p->prefix_splits > 65536 || p->own_splits > 65536 || (p->P > 0 && p->prefix_splits < 1) ||
+      (p->S > 0 && p->own_splits < 1) || p->prefix_splits + p->own_splits < 1)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: splits must be in [0, 65536], and at least 1 for a part with keys");
+  if (!(p->scale > 0.f) || !(p->scale * kLog2e < INFINITY)) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: scale must be positive and finite");
+  const int64_t strides[16] = {p->q_seq, p->q_row, p->q_head, p->kp_row, p->kp_head, p->vp_row, p->vp_head, p->ko_seq,
+                               p->ko_row, p->ko_head, p->vo_seq, p->vo_row, p->vo_head, p->out_seq, p->out_row, p->out_head};
+  for (int i = 0; i < 16; ++i)
+    if (strides[i] < 0 || strides[i] % e) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: strides must be >= 0 and keep rows 16-byte aligned");
+  if (((uintptr_t)p->q | (uintptr_t)p->kp | (uintptr_t)p->vp | (uintptr_t)p->ko | (uintptr_t)p->vo | (uintptr_t)p->out | (uintptr_t)p->scratch) % 16)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: tensors must be 16-byte aligned");
+  if (p->B == 0 || p->L == 0) return PP_OK;  // no row to write
+  PrefixK a;
+  a.q = p->q; a.kp = p->kp; a.vp = p->vp; a.ko = p->ko; a.vo = p->vo; a.out = p->out; a.own_len = (const int*)p->own_len;
+  a.q_seq = p->q_seq; a.q_row = p->q_row; a.q_head = p->q_head;
+  a.kp_row = p->kp_row; a.kp_head = p->kp_head; a.vp_row = p->vp_row; a.vp_head = p->vp_head;
+  a.ko_seq = p->ko_seq; a.ko_row = p->ko_row; a.ko_head = p->ko_head;
+  a.vo_seq = p->vo_seq; a.vo_row = p->vo_row; a.vo_head = p->vo_head;
+  a.out_seq = p->out_seq; a.out_row = p->out_row; a.out_head = p->out_head;
+  a.P = p->P; a.S = p->S;
+  a.B = (int)p->B; a.L = (int)p->L; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D;
+  a.prefix_splits = p->P > 0 ? p->prefix_splits : 0;
+  a.own_splits = p->S > 0 ? p->own_splits : 0;
+  a.parts = a.prefix_splits + a.own_splits;
+  a.sc = p->scale * kLog2e;
+  const int64_t rows = p->B * p->L * p->H;
+  if (rows > ((int64_t)1 << 40) / 65536 || p->L * a.G > INT32_MAX / 2) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: too many rows");
+  if (p->scratch_bytes < rows * (p->prefix_splits + p->own_splits) * (p->D + 4) * 4)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: scratch smaller than B * L * H * (prefix_splits + own_splits) * (D + 4) floats");
+  a.part_o = (float*)p->scratch;
+  a.part_ml = a.part_o + rows * a.parts * p->D;
+  a.prefix_tiles = (int)((rows / a.KH + kRows - 1) / kRows);
+  a.own_tiles = (int)(((int64_t)a.L * a.G + kRows - 1) / kRows);
+  a.prefix_items = (int64_t)a.prefix_splits * a.prefix_tiles * a.KH;
+  if (p->dtype == PP_F32) return launch_prefix_d<float>(stream, a);
+  if (p->dtype == PP_F16) return launch_prefix_d<half_t>(stream, a);
+  return launch_prefix_d<bf16_t>(stream, a);
+}

@@ -1,0 +1,144 @@
+// prompt_attention.hip -- attention over packed sequences of different lengths, grouped heads, causal or not.
+// Contract: include/propainter_mi355.h (pp_prompt_attention); the inner loop: tile_attention.h.
+//
+// The n query tokens of a sequence and the G = H / KH query heads of a key / value head make n * G rows, row = token * G + head in the group:
+// a work-group takes 128 of them, so short prompts fill its tiles with heads, and the keys of a group are staged once for all of its heads.
+// Tiles are numbered without knowing a length on the host: sequence s starts at tile floor(cu_q[s] G / 128) + s, which leaves each at
+// least ceil(n G / 128) numbers; a work-group finds its sequence by a 64-ary search over cu_q and returns if its number is spare.
+// Later tiles of a causal sequence see more keys and are launched first; the key / value head is the fastest index of the grid, so with 8 (or a
+// multiple or divisor of 8) of them a head's keys stay in the L2 of its XCDs.
+#include "tile_attention.h"
+#include "pp_host.h"
+
+#include <math.h>
+
+namespace pp {
+
+struct PromptK {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int *cu_q, *cu_k;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, Tq, Tk;
+  int B, H, KH, G, D, causal, ntiles;
+  float scale, sc;
+};
+
+constexpr int kRows = 128;
+
+__device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
+  const int64_t v = cu[i];
+  return v < 0 ? 0 : v > most ? most : v;
+}
+
+template <typename Tile>
+__global__ void __launch_bounds__(256) prompt_attention_kernel(const PromptK a) {
+  typedef typename Tile::type T;
+  const int kh = (int)blockIdx.x % a.KH;
+  const int64_t tile = a.ntiles - 1 - (int)blockIdx.x / a.KH;
+  const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
+
+  // ---- the sequence that owns this tile: the last s with first_tile(s) <= tile
+  int s = 0;
+  for (int n = a.B; n > 1;) {
+    const int step = (n + 63) / 64, i = s + lane * step;
+    const bool below = lane * step < n && (lane == 0 || clamped(a.cu_q, i, a.Tq) * a.G / kRows + i <= tile);
+    const int count = wave_count(below);
+    s += (count - 1) * step;
+    n = n - (count - 1) * step < step ? n - (count - 1) * step : step;
+  }
+  const int64_t q0 = clamped(a.cu_q, s, a.Tq), q1 = clamped(a.cu_q, s + 1, a.Tq);
+  const int64_t k0 = clamped(a.cu_k, s, a.Tk), k1 = clamped(a.cu_k, s + 1, a.Tk);
+  const int64_t n = q1 - q0, m = k1 > k0 ? k1 - k0 : 0, rows = n * a.G;
+  const int64_t row0 = (tile - (q0 * a.G / kRows + s)) * kRows;
+  if (row0 < 0 || row0 >= rows) return;
+
+  // ---- what this lane's row, its wave and the work-group see
+  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int64_t {
+    if (!a.causal) return m;
+    const int64_t c = row / a.G + 1 + m - n;
+    return c < 0 ? 0 : c > m ? m : c;
+  };
+  const int64_t last = rows - 1;
+  const int64_t wrow = row0 + 32 * wave, row = wrow + q32;
+  const bool live = row <= last;
+  const int64_t limit = live ? limit_of(row) : 0;
+  const int64_t wave_min = wrow <= last ? limit_of(wrow) : 0;
+  const int64_t wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
+  const int64_t nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
+
+  const int64_t token = q0 + (live ? row / a.G : 0);
+  const int head = kh * a.G + (live ? (int)(row % a.G) : 0);
+  Tile t;
+  AttnState<Tile> st;
+  t.init(PP_DYN_SMEM);
+  t.load_q(live ? (const T*)a.q + token * a.q_row + head * a.q_head : nullptr, a.D);
+  attend(t, st, (const T*)a.k + k0 * a.k_row + kh * a.k_head, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.k_row, a.v_row, nkeys, limit,
+         wave_min, wave_max, a.D, a.sc);
+  if (!live) return;
+  // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
+  const float inv = limit > 0 ? 1.f / st.l : 0.f;
+  T* dst = (T*)a.out + token * a.out_row + head * a.out_head;
+#pragma unroll
+  for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * db + 8 * g + 4 * h;
+      if (d < a.D)
+        Tile::store4(dst + d, st.o[db][4 * g] * inv, st.o[db][4 * g + 1] * inv, st.o[db][4 * g + 2] * inv, st.o[db][4 * g + 3] * inv);
+    }
+  if (a.lse && h == 0) a.lse[token * a.H + head] = limit > 0 ? st.m * a.scale + logf(st.l) : neg_inf();
+}
+
+}  // namespace pp
+
+template <typename T, int DP>
+static int launch_prompt(void* stream, const pp::PromptK& a) {
+  using namespace pp;
+  typedef AttnTile<T, DP> Tile;
+  PP_ALLOW_BIG_LDS((&prompt_attention_kernel<Tile>), Tile::kSmem);
+  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH)), dim3(256), Tile::kSmem, stream, a);
+  return pp_check_launch("pp_prompt_attention");
+}
+
+template <typename T>
+static int launch_prompt_d(void* stream, const pp::PromptK& a) {
+  if (a.D <= 32) return launch_prompt<T, 32>(stream, a);
+  if (a.D <= 64) return launch_prompt<T, 64>(stream, a);
+  if (a.D <= 96) return launch_prompt<T, 96>(stream, a);
+  if (a.D <= 128) return launch_prompt<T, 128>(stream, a);
+  return launch_prompt<T, 256>(stream, a);
+}
+
+extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p) {
+  using namespace pp;
+  if (!p || !p->q || !p->k || !p->v || !p->out || !p->cu_q || !p->cu_k) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: null argument");
+  if (p->dtype != PP_F32 && p->dtype != PP_F16 && p->dtype != PP_BF16) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: dtype");
+  if (p->KH < 1 || p->H < 1 || p->H % p->KH || p->H > (1 << 20))
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: H must be a multiple of KH");
+  const int e = p->dtype == PP_F32 ? 4 : 8;  // elements of 16 bytes
+  if (p->D < 1 || p->D > 256 || p->D % e) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: D must be a multiple of 8 (fp32: 4) up to 256");
+  if (p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->B > INT32_MAX / 2 || p->Tq > INT32_MAX || p->Tk > INT32_MAX)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: B, Tq, Tk must be in [0, 2^31)");
+  if (!(p->scale > 0.f) || !(p->scale * kLog2e < INFINITY)) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: scale must be positive and finite");
+  const int64_t strides[8] = {p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head, p->out_row, p->out_head};
+  for (int i = 0; i < 8; ++i)
+    if (strides[i] < 0 || strides[i] % e) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: strides must be >= 0 and keep rows 16-byte aligned");
+  if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) % 16)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: tensors must be 16-byte aligned");
+  if (p->B == 0 || p->Tq == 0) return PP_OK;  // no row to write
+  PromptK a;
+  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = (float*)p->lse;
+  a.cu_q = (const int*)p->cu_q; a.cu_k = (const int*)p->cu_k;
+  a.q_row = p->q_row; a.q_head = p->q_head; a.k_row = p->k_row; a.k_head = p->k_head;
+  a.v_row = p->v_row; a.v_head = p->v_head; a.out_row = p->out_row; a.out_head = p->out_head;
+  a.Tq = p->Tq; a.Tk = p->Tk;
+  a.B = (int)p->B; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D; a.causal = p->causal != 0;
+  a.scale = p->scale; a.sc = p->scale * kLog2e;
+  const int64_t ntiles = p->Tq * a.G / kRows + p->B;
+  if (ntiles * p->KH * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
+  a.ntiles = (int)ntiles;
+  if (p->dtype == PP_F32) return launch_prompt_d<float>(stream, a);
+  if (p->dtype == PP_F16) return launch_prompt_d<half_t>(stream, a);
+  return launch_prompt_d<bf16_t>(stream, a);
+}

@@ -37,6 +37,9 @@ EPI = {
     "add_relu": _lib.CONSTS["PP_EPI_ADD_AUX1_RELU"],
     "gru": _lib.CONSTS["PP_EPI_GRU"],
 }
+# activations of groupnorm (the convolutions' epilogues know all of them but silu)
+NORM_ACT = {**ACT, "silu": _lib.CONSTS["PP_ACT_SILU"]}
+_LM_DTYPE = {torch.float32: PP_F32, torch.float16: PP_F16, torch.bfloat16: _lib.CONSTS["PP_BF16"]}
 PAD = {"zeros": _lib.CONSTS["PP_PAD_ZEROS"], "replicate": _lib.CONSTS["PP_PAD_REPLICATE"]}
 
 
@@ -651,6 +654,65 @@ def instnorm(x: torch.Tensor, y: torch.Tensor, *, relu_pre=False, relu_post=Fals
     return y
 
 
+def _lm_dtype(name: str, *tensors) -> int:
+    """dtype code of the operators that also take bfloat16 (groupnorm, prompt_attention, prefix_attention); one dtype for all tensors."""
+    dt = tensors[0].dtype
+    code = _LM_DTYPE.get(dt)
+    if code is None:
+        raise TypeError(f"{name}: unsupported dtype {dt} (float16, bfloat16 or float32)")
+    for t in tensors[1:]:
+        if t is not None and t.dtype != dt:
+            raise TypeError(f"{name}: tensors must share a dtype, got {dt} and {t.dtype}")
+    return code
+
+
+def groupnorm(x: torch.Tensor, y: torch.Tensor, groups: int, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, *,
+              act=None, act_param: float = 0.0, skip: torch.Tensor | None = None, relu_post: bool = False, eps: float = 1e-5,
+              scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """y = post(skip + act(groupnorm(x))) on channels-last f16 / bf16 / fp32 [N,H,W,C] views; groups of C // groups channels, fp32
+    gamma / beta [C] (or None), statistics in double, post = ReLU if `relu_post`.  act: a key of NORM_ACT.  y may be x or skip.
+    `scratch`: float64, groupnorm_scratch() elements; by default a tensor of this call's own, so that two captured graphs or two
+    streams never share one.  A caller that passes its own must not let two calls run on it at once."""
+    check_device(x, y, gamma, beta, skip)
+    n, h, w, c, x_ldc = nhwc_view(x)
+    if y.shape != x.shape or (skip is not None and skip.shape != x.shape):
+        raise ValueError("groupnorm: x, y and skip must share a shape")
+    code = _lm_dtype("groupnorm", x, y, skip)
+    if groups < 1 or c % groups:
+        raise ValueError(f"groupnorm: {c} channels are not a multiple of {groups} groups")
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous()):
+            raise ValueError(f"groupnorm: {name} must be a dense fp32 [{c}] tensor")
+    if act not in NORM_ACT:
+        raise ValueError(f"groupnorm: unknown activation {act!r}")
+    need, nchunks = groupnorm_scratch(n, h * w, c, groups, x.element_size())
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.float64, device=x.device)
+    else:
+        check_device(scratch)
+        if scratch.dtype != torch.float64 or scratch.numel() < need or not scratch.is_contiguous():
+            raise ValueError(f"groupnorm: scratch must be a dense float64 tensor of at least {need} elements")
+    P = _lib.STRUCTS["pp_groupnorm_params"]()
+    P.dtype, P.act, P.act_param, P.relu_post, P.eps = code, NORM_ACT[act], act_param, int(relu_post), eps
+    P.x, P.x_ldc, P.y, P.y_ldc = x.data_ptr(), x_ldc, y.data_ptr(), nhwc_view(y)[4]
+    if skip is not None:
+        P.skip, P.skip_ldc = skip.data_ptr(), nhwc_view(skip)[4]
+    P.gamma = gamma.data_ptr() if gamma is not None else None
+    P.beta = beta.data_ptr() if beta is not None else None
+    P.N, P.HW, P.C, P.groups = n, h * w, c, groups
+    P.partials, P.nchunks = scratch.data_ptr(), nchunks
+    if n * h * w > 0:
+        _call("pp_groupnorm", y, P)
+    return y
+
+
+def groupnorm_scratch(n: int, hw: int, c: int, groups: int, element_size: int) -> tuple[int, int]:
+    """(float64 elements of scratch, pieces per image) of a groupnorm call."""
+    # pieces of at least 32 KiB, and about 2048 work-groups (8 per CU) over all images
+    nchunks = max(1, min(hw, hw * c * element_size // 32768, -(-2048 // max(1, n))))
+    return max(2, (nchunks + 1) * n * groups * 2), nchunks
+
+
 def tiled_pitch(h: int, w: int) -> int:
     """Floats of an h x w correlation plane stored in 4 x 8 tiles of 128 bytes (pp_corr_lookup)."""
     return -(-h // 4) * -(-w // 8) * 32
@@ -1076,6 +1138,126 @@ def window_attention(qkv: torch.Tensor, pkv: torch.Tensor, win_masked: torch.Ten
     else:
         _call("pp_window_attention", out, P)
     return out
+
+
+def _heads_view(name: str, t: torch.Tensor, dims: int) -> tuple:
+    """Element strides of a [..., heads, D] view (0 for dims of one element, whose stride says nothing)."""
+    if t.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dims, got {tuple(t.shape)}")
+    st, sh = t.stride(), t.shape
+    if st[-1] != 1 and sh[-1] > 1:
+        raise ValueError(f"{name}: the last dim must be dense, got strides {st}")
+    return tuple(a if n > 1 else 0 for a, n in zip(st[:-1], sh[:-1]))
+
+
+def _writable(name: str, t: torch.Tensor) -> None:
+    if any(a == 0 and n > 1 for a, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name}: an expanded view cannot be written")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
+                     lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over packed sequences: q, out [Tq,H,D], k, v [Tk,KH,D] (any strides, dense last dim; f16 / bf16 / fp32), H a multiple of
+    KH; sequence s = query rows cu_q[s]:cu_q[s+1] and key rows cu_k[s]:cu_k[s+1] (i32 on the device; cu_k None: cu_q).  causal: query i of
+    n sees key j of m if j <= i + m - n.  A query without a key gets 0; rows outside every sequence are left as they were.
+    scale: 1/sqrt(D) by default.  lse: fp32 [Tq,H], ln of the softmax sums (-inf without a key).  out may be q; it must not overlap
+    k or v."""
+    cu_k = cu_q if cu_k is None else cu_k
+    check_device(q, k, v, out, cu_q, cu_k, lse)
+    qs, ks, vs, os_ = _heads_view("q", q, 3), _heads_view("k", k, 3), _heads_view("v", v, 3), _heads_view("out", out, 3)
+    tq, h, d = q.shape
+    tk, kh, _ = k.shape
+    if out.shape != q.shape or v.shape != k.shape or k.shape[2] != d or kh < 1 or h < 1 or h % kh:
+        raise ValueError(f"prompt_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
+    code = _lm_dtype("prompt_attention", q, k, v, out)
+    _writable("out", out)
+    for name, t in (("cu_q", cu_q), ("cu_k", cu_k)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != cu_q.numel() or t.numel() < 1 or not t.is_contiguous():
+            raise ValueError(f"prompt_attention: {name} must be a dense int32 [sequences + 1] tensor")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tq, h) or not lse.is_contiguous()):
+        raise ValueError(f"prompt_attention: lse must be a dense fp32 [{tq}, {h}] tensor")
+    P = _lib.STRUCTS["pp_prompt_attention_params"]()
+    P.dtype, P.causal, P.scale = code, int(causal), d ** -0.5 if scale is None else scale
+    P.q, P.q_row, P.q_head = q.data_ptr(), qs[0], qs[1]
+    P.k, P.k_row, P.k_head = k.data_ptr(), ks[0], ks[1]
+    P.v, P.v_row, P.v_head = v.data_ptr(), vs[0], vs[1]
+    P.out, P.out_row, P.out_head = out.data_ptr(), os_[0], os_[1]
+    P.lse = lse.data_ptr() if lse is not None else None
+    P.cu_q, P.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    P.B, P.Tq, P.Tk, P.H, P.KH, P.D = cu_q.numel() - 1, tq, tk, h, kh, d
+    if tq > 0:
+        if tk == 0:          # every row is empty; an empty tensor has no address
+            P.k = P.v = P.q
+        _call("pp_prompt_attention", out, P)
+    return out
+
+
+def prefix_splits(b: int, new: int, p: int, s: int, h: int, kh: int) -> tuple[int, int]:
+    """(pieces of the prefix, pieces of an own range) of a prefix_attention call."""
+    tiles = -(-b * new * (h // kh) // 128) * kh
+    own = -(-new * (h // kh) // 128) * kh * b
+    # 512 work-groups fill the chip twice over; a piece has at least 256 keys
+    return (max(1, min(-(-p // 256), 512 // max(1, tiles))) if p else 0), (max(1, min(-(-s // 256), 512 // max(1, own))) if s else 0)
+
+
+def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_own: torch.Tensor, v_own: torch.Tensor,
+                     own_len: torch.Tensor, out: torch.Tensor, *, scale: float | None = None,
+                     scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the newest tokens of a batch of sequences behind a shared prefix: q, out [B,L,H,D] (or [B,H,D]: one token each),
+    k_prefix, v_prefix [P,KH,D], k_own, v_own [B,S,KH,D] (any strides, dense last dim; f16 / bf16 / fp32), own_len i32 [B] on the
+    device: keys of a sequence behind the prefix, its L new tokens among them.  Token i of L sees the prefix and own keys
+    j <= own_len[b] - L + i; a row without a key gets 0.  P and S may be 0.  scale: 1/sqrt(D) by default.
+    `scratch`: float32, prefix_attention_scratch() elements; by default a tensor of this call's own, so that two captured graphs or two
+    streams never share one.  A caller that passes its own must not let two calls run on it at once.  out may be q; it must not overlap the keys or values."""
+    if q.dim() == 3 and out.dim() == 3:
+        prefix_attention(q.unsqueeze(1), k_prefix, v_prefix, k_own, v_own, own_len, out.unsqueeze(1), scale=scale, scratch=scratch)
+        return out
+    check_device(q, k_prefix, v_prefix, k_own, v_own, own_len, out)
+    qs, os_ = _heads_view("q", q, 4), _heads_view("out", out, 4)
+    kps, vps = _heads_view("k_prefix", k_prefix, 3), _heads_view("v_prefix", v_prefix, 3)
+    kos, vos = _heads_view("k_own", k_own, 4), _heads_view("v_own", v_own, 4)
+    b, new, h, d = q.shape
+    p, kh, _ = k_prefix.shape
+    s = k_own.shape[1]
+    if (out.shape != q.shape or v_prefix.shape != k_prefix.shape or v_own.shape != k_own.shape or k_prefix.shape[2] != d
+            or k_own.shape != (b, s, kh, d) or kh < 1 or h < 1 or h % kh):
+        raise ValueError(f"prefix_attention: shapes q {tuple(q.shape)}, prefix {tuple(k_prefix.shape)} / {tuple(v_prefix.shape)}, own "
+                         f"{tuple(k_own.shape)} / {tuple(v_own.shape)}, out {tuple(out.shape)}")
+    code = _lm_dtype("prefix_attention", q, k_prefix, v_prefix, k_own, v_own, out)
+    _writable("out", out)
+    if own_len.dtype != torch.int32 or own_len.shape != (b,) or not own_len.is_contiguous():
+        raise ValueError(f"prefix_attention: own_len must be a dense int32 [{b}] tensor")
+    ps, osp = prefix_splits(b, new, p, s, h, kh)
+    need = prefix_attention_scratch(q, k_prefix, k_own)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    else:
+        check_device(scratch)
+        if scratch.dtype != torch.float32 or scratch.numel() < need or not scratch.is_contiguous():
+            raise ValueError(f"prefix_attention: scratch must be a dense float32 tensor of at least {need} elements")
+    P = _lib.STRUCTS["pp_prefix_attention_params"]()
+    P.dtype, P.prefix_splits, P.own_splits, P.scale = code, ps, osp, d ** -0.5 if scale is None else scale
+    if ps + osp == 0:
+        P.prefix_splits = 1
+    P.q, P.q_seq, P.q_row, P.q_head = q.data_ptr(), *qs
+    P.kp, P.kp_row, P.kp_head = k_prefix.data_ptr(), *kps
+    P.vp, P.vp_row, P.vp_head = v_prefix.data_ptr(), *vps
+    P.ko, P.ko_seq, P.ko_row, P.ko_head = k_own.data_ptr(), *kos
+    P.vo, P.vo_seq, P.vo_row, P.vo_head = v_own.data_ptr(), *vos
+    P.own_len = own_len.data_ptr()
+    P.out, P.out_seq, P.out_row, P.out_head = out.data_ptr(), *os_
+    P.scratch, P.scratch_bytes = scratch.data_ptr(), scratch.numel() * 4
+    P.B, P.L, P.P, P.S, P.H, P.KH, P.D = b, new, p, s, h, kh, d
+    if b * new > 0:
+        _call("pp_prefix_attention", out, P)
+    return out
+
+
+def prefix_attention_scratch(q: torch.Tensor, k_prefix: torch.Tensor, k_own: torch.Tensor) -> int:
+    """float32 elements of scratch of a prefix_attention call on these tensors."""
+    b, new, h, d = q.shape if q.dim() == 4 else (q.shape[0], 1, *q.shape[1:])
+    return max(4, b * new * h * max(1, sum(prefix_splits(b, new, k_prefix.shape[0], k_own.shape[1], h, k_prefix.shape[1]))) * (d + 4))
 
 
 def fold(x: torch.Tensor, out: torch.Tensor, fh: int, fw: int, normalize: bool, gelu: bool = False) -> torch.Tensor:

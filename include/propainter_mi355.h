@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define PP_ABI_VERSION 12
+#define PP_ABI_VERSION 13
 
 enum pp_dtype {
   PP_F32 = 0,
@@ -42,7 +42,8 @@ enum pp_dtype {
    * subnormals --, three MFMAs per product into one fp32 accumulator: |v - h - l| <= max(2^-20 |v|, 2^-24); beyond the f16
    * range both terms saturate: |v| <= 131008 is representable to <= 32 absolute, larger values saturate, never Inf/NaN).
    * Weights must be in the split packing described at pp_conv2d. */
-  PP_F32X2 = 4
+  PP_F32X2 = 4,
+  PP_BF16 = 5 /* (ABI v13) pp_groupnorm, pp_prompt_attention and pp_prefix_attention only */
 };
 
 enum pp_status {
@@ -52,7 +53,8 @@ enum pp_status {
   PP_ERR_LAUNCH = -3
 };
 
-enum pp_act { PP_ACT_NONE = 0, PP_ACT_RELU = 1, PP_ACT_LEAKY = 2, PP_ACT_SIGMOID = 3, PP_ACT_TANH = 4, PP_ACT_GELU = 5 };
+enum pp_act { PP_ACT_NONE = 0, PP_ACT_RELU = 1, PP_ACT_LEAKY = 2, PP_ACT_SIGMOID = 3, PP_ACT_TANH = 4, PP_ACT_GELU = 5,
+              PP_ACT_SILU = 6 /* (ABI v13) pp_groupnorm only: x * sigmoid(x) */ };
 
 enum pp_epilogue {
   PP_EPI_NONE = 0,
@@ -506,6 +508,101 @@ typedef struct {
                     at fp32 rounding level, ~5x the time of the default; 0 = f16 MFMA operands.  Must be 0 for PP_F16. */
 } pp_window_attention_params;
 int32_t pp_window_attention(void* stream, const pp_window_attention_params* p);
+
+/* ------------------------------------------------------------------------------------
+ * pp_groupnorm (ABI v13) -- group norm fused with an activation and an optional residual, channels-last:
+ *   group g of image n = its HW pixels x C/groups channels; mean, var over the group (biased, accumulated in double);
+ *   y = post( skip + act( (x - mean) / sqrt(var + eps) * gamma[c] + beta[c] ) ),  post = relu if relu_post.
+ * RAFT's encoders offer it as norm_fn = "group" next to "instance" and "batch" (groups of 8 channels).
+ * `partials`: caller-owned scratch of (nchunks + 1) * N * groups * 2 doubles (16-byte aligned); nchunks in [1, HW]: pieces
+ * of an image that the statistics pass deals to work-groups.  The result depends on nchunks only by the order of double sums.
+ * y may be x (in place) or skip; x, y and skip share dtype; gamma / beta may be NULL (1 / 0).
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  int32_t dtype; /* x, y, skip: PP_F32, PP_F16 or PP_BF16 */
+  int32_t act;   /* pp_act, PP_ACT_SILU included */
+  const void* x;
+  int64_t x_ldc;
+  void* y;
+  int64_t y_ldc;
+  const void* skip; /* optional residual input (same shape), NULL = none */
+  int64_t skip_ldc;
+  const void* gamma; /* fp32 [C] or NULL */
+  const void* beta;  /* fp32 [C] or NULL */
+  int64_t N, HW, C, groups;
+  void* partials;
+  int64_t nchunks;
+  float eps;
+  float act_param; /* leaky slope */
+  int32_t relu_post;
+} pp_groupnorm_params;
+int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p);
+
+/* ------------------------------------------------------------------------------------
+ * pp_prompt_attention (ABI v13) -- attention over packed sequences of different lengths, grouped heads, online softmax:
+ *   sequence s owns query rows cu_q[s] .. cu_q[s+1]-1 and key rows cu_k[s] .. cu_k[s+1]-1; query head h reads key / value
+ *   head h / (H / KH); with n query and m key rows, query i sees key j if !causal or j <= i + (m - n);
+ *   out = softmax_j(scale * q . k_j) v_j;  lse (optional) = ln sum_j exp(scale * q . k_j).
+ * A query that sees no key gets out = 0, lse = -inf.  Query rows outside every sequence are not written.  Keys, values and queries
+ * that a row does not see never reach its result, whatever they hold (NaN and infinities included).
+ * The offsets live on the device: values outside [0, Tq] / [0, Tk] are clamped, a sequence of negative length is empty.
+ * Strides in elements; the last dim is dense; every row start is 16-byte aligned; D % 8 == 0 (% 4 for PP_F32), D <= 256.
+ * PP_F16 / PP_BF16: MFMA operands in the storage type (the probabilities are rounded to it once, as operands of the second
+ * product), fp32 scores, sums and accumulators.  PP_F32: everything fp32 (f32 MFMA).
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  int32_t dtype; /* q, k, v, out: PP_F32, PP_F16 or PP_BF16 */
+  int32_t causal;
+  const void* q;
+  int64_t q_row, q_head; /* strides: token, head */
+  const void* k;
+  int64_t k_row, k_head;
+  const void* v;
+  int64_t v_row, v_head;
+  void* out;
+  int64_t out_row, out_head;
+  void* lse;        /* fp32 [Tq][H] dense, or NULL */
+  const void* cu_q; /* i32 [B + 1] */
+  const void* cu_k; /* i32 [B + 1] */
+  int64_t B, Tq, Tk, H, KH, D;
+  float scale; /* > 0, finite */
+} pp_prompt_attention_params;
+int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p);
+
+/* ------------------------------------------------------------------------------------
+ * pp_prefix_attention (ABI v13) -- attention of a batch of sequences that share a prefix: the L newest tokens of each of B
+ * sequences against the P shared prefix keys and the sequence's own keys, one softmax over both.
+ *   q, out [B][L][H][D]; kp, vp [P][KH][D]; ko, vo [B][S][KH][D]; own_len i32 [B] (on the device; clamped to [0, S]): keys of
+ *   sequence b behind the prefix, its L new tokens among them.  Token i of L sees the whole prefix and own keys
+ *   j <= own_len[b] - L + i.  A row that sees no key gets 0.  Keys and values that a row does not see never reach its result.
+ * The prefix's keys and values are read once for all rows of a key / value head, not once per sequence.
+ * `scratch`: caller-owned, 16-byte aligned, B * L * H * (prefix_splits + own_splits) * (D + 4) floats; prefix_splits pieces of the
+ * prefix and own_splits pieces of each own range go to different work-groups and are joined in a fixed order (both >= 0, a
+ * part with keys needs at least one).  Strides in elements as in pp_prompt_attention.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  int32_t dtype; /* q, kp, vp, ko, vo, out: PP_F32, PP_F16 or PP_BF16 */
+  int32_t prefix_splits;
+  int32_t own_splits;
+  float scale; /* > 0, finite */
+  const void* q;
+  int64_t q_seq, q_row, q_head; /* strides: sequence, token, head */
+  const void* kp;
+  int64_t kp_row, kp_head;
+  const void* vp;
+  int64_t vp_row, vp_head;
+  const void* ko;
+  int64_t ko_seq, ko_row, ko_head;
+  const void* vo;
+  int64_t vo_seq, vo_row, vo_head;
+  const void* own_len; /* i32 [B] */
+  void* out;
+  int64_t out_seq, out_row, out_head;
+  void* scratch;
+  int64_t scratch_bytes;
+  int64_t B, L, P, S, H, KH, D;
+} pp_prefix_attention_params;
+int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_params* p);
 
 /* ------------------------------------------------------------------------------------
  * pp_fold / pp_unfold_gelu -- F.fold / F.unfold with kernel 7, stride 3, padding 3
