@@ -26,11 +26,10 @@ struct PrefixK {
   float sc;
 };
 
-constexpr int kRows = 128;
-
 template <typename Tile>
-__global__ void __launch_bounds__(256) prefix_attention_kernel(const PrefixK a) {
+__global__ void __launch_bounds__(256, Tile::kWaves) prefix_attention_kernel(const PrefixK a) {
   typedef typename Tile::type T;
+  constexpr int kRows = Tile::kRows, RB = Tile::RB;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
   const bool shared = (int64_t)blockIdx.x < a.prefix_items;
   int64_t id = shared ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - a.prefix_items;
@@ -70,41 +69,50 @@ __global__ void __launch_bounds__(256) prefix_attention_kernel(const PrefixK a) 
     v_row = a.vo_row;
   }
   // keys of [n0, n1) that a row sees
-  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int64_t {
-    if (shared) return n1 - n0;
-    const int64_t c = visible - a.L + row / a.G + 1 - n0;
-    return c < 0 ? 0 : c > n1 - n0 ? n1 - n0 : c;
+  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int {
+    const int64_t c = shared ? n1 - n0 : visible - a.L + row / a.G + 1 - n0;
+    return (int)(c < 0 ? 0 : c > n1 - n0 ? n1 - n0 : c);
   };
-  const int64_t last = rows - 1;
-  const int64_t wrow = row0 + 32 * wave, row = wrow + q32;
-  const bool live = row <= last;
-  const int64_t limit = live ? limit_of(row) : 0;
-  const int64_t wave_min = wrow <= last ? limit_of(wrow) : 0;
-  const int64_t wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
-  const int64_t nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
-
-  const int64_t r = live ? row : 0;
-  const int64_t b = shared ? r / lg : seq;
-  const int in_seq = (int)(shared ? r % lg : r);
-  const int tok = in_seq / a.G, head = kh * a.G + in_seq % a.G;
+  const int64_t last = rows - 1, wrow = row0 + 32 * RB * wave;
+  AttnLimits<RB> lim;
+  lim.wave_min = wrow <= last ? limit_of(wrow) : 0;
+  lim.wave_max = wrow <= last ? limit_of(wrow + 32 * RB - 1 < last ? wrow + 32 * RB - 1 : last) : 0;
+  lim.group_min = limit_of(row0);
+  lim.nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
   Tile t;
   AttnState<Tile> st;
   t.init(PP_DYN_SMEM);
-  t.load_q(live ? (const T*)a.q + b * a.q_seq + tok * a.q_row + head * a.q_head : nullptr, a.D);
-  attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, nkeys, limit, wave_min, wave_max, a.D, a.sc);
-  if (!live) return;
-  const int64_t at = ((b * a.L + tok) * a.H + head) * a.parts + part;
-  float* dst = a.part_o + at * a.D;
 #pragma unroll
-  for (int db = 0; db < Tile::kDB; ++db)
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t row = wrow + 32 * rb + q32;
+    const bool live = row <= last;
+    lim.row[rb] = live ? limit_of(row) : 0;
+    const int64_t b = shared ? row / lg : seq;
+    const int in_seq = (int)(shared ? row % lg : row);
+    t.load_q(rb, live ? (const T*)a.q + b * a.q_seq + (in_seq / a.G) * a.q_row + (kh * a.G + in_seq % a.G) * a.q_head : nullptr, a.D);
+  }
+  attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, lim, a.D, a.sc);
+  if (st.not_finite) add_not_finite(t, st, v + n0 * v_row, v_row, lim, a.D);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * db + 8 * g + 4 * h;
-      if (d < a.D) *reinterpret_cast<f4*>(dst + d) = f4{st.o[db][4 * g], st.o[db][4 * g + 1], st.o[db][4 * g + 2], st.o[db][4 * g + 3]};
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t row = wrow + 32 * rb + q32;
+    if (row > last) continue;
+    const int64_t b = shared ? row / lg : seq;
+    const int in_seq = (int)(shared ? row % lg : row);
+    const int64_t at = ((b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G) * a.parts + part;
+    float* dst = a.part_o + at * a.D;
+#pragma unroll
+    for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * db + 8 * g + 4 * h;
+        const f16v& o = st.o[rb][db];
+        if (d < a.D) *reinterpret_cast<f4*>(dst + d) = f4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
+      }
+    if (h == 0) {
+      a.part_ml[2 * at] = st.m[rb];
+      a.part_ml[2 * at + 1] = st.l[rb];
     }
-  if (h == 0) {
-    a.part_ml[2 * at] = st.m;
-    a.part_ml[2 * at + 1] = st.l;
   }
 }
 
@@ -138,10 +146,13 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixK a) {
 
 }  // namespace pp
 
-template <typename T, int DP>
-static int launch_prefix(void* stream, const pp::PrefixK& a) {
+template <typename Tile>
+static int launch_prefix(void* stream, pp::PrefixK& a) {
   using namespace pp;
-  typedef AttnTile<T, DP> Tile;
+  const int64_t rows = (int64_t)a.B * a.L * a.G;
+  a.prefix_tiles = (int)((rows + Tile::kRows - 1) / Tile::kRows);
+  a.own_tiles = (a.L * a.G + Tile::kRows - 1) / Tile::kRows;
+  a.prefix_items = (int64_t)a.prefix_splits * a.prefix_tiles * a.KH;
   const int64_t items = a.prefix_items + (int64_t)a.own_splits * a.B * a.own_tiles * a.KH;
   if (items * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the launch needs 2^32 threads or more");
   PP_ALLOW_BIG_LDS((&prefix_attention_kernel<Tile>), Tile::kSmem);
@@ -153,12 +164,17 @@ static int launch_prefix(void* stream, const pp::PrefixK& a) {
 }
 
 template <typename T>
-static int launch_prefix_d(void* stream, const pp::PrefixK& a) {
-  if (a.D <= 32) return launch_prefix<T, 32>(stream, a);
-  if (a.D <= 64) return launch_prefix<T, 64>(stream, a);
-  if (a.D <= 96) return launch_prefix<T, 96>(stream, a);
-  if (a.D <= 128) return launch_prefix<T, 128>(stream, a);
-  return launch_prefix<T, 256>(stream, a);
+static int launch_prefix_d(void* stream, pp::PrefixK& a) {
+  using namespace pp;
+  if constexpr (sizeof(T) == 2) {
+    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 2>>(stream, a);
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 2>>(stream, a);
+  }
+  if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 1>>(stream, a);
+  if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 1>>(stream, a);
+  if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 1, 1>>(stream, a);
+  if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 1, 1>>(stream, a);
+  return launch_prefix<AttnTile<T, 256, 1, 1>>(stream, a);
 }
 
 extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_params* p) {
@@ -202,9 +218,6 @@ extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_p
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: scratch smaller than B * L * H * (prefix_splits + own_splits) * (D + 4) floats");
   a.part_o = (float*)p->scratch;
   a.part_ml = a.part_o + rows * a.parts * p->D;
-  a.prefix_tiles = (int)((rows / a.KH + kRows - 1) / kRows);
-  a.own_tiles = (int)(((int64_t)a.L * a.G + kRows - 1) / kRows);
-  a.prefix_items = (int64_t)a.prefix_splits * a.prefix_tiles * a.KH;
   if (p->dtype == PP_F32) return launch_prefix_d<float>(stream, a);
   if (p->dtype == PP_F16) return launch_prefix_d<half_t>(stream, a);
   return launch_prefix_d<bf16_t>(stream, a);

@@ -2,9 +2,9 @@
 // Contract: include/propainter_mi355.h (pp_prompt_attention); the inner loop: tile_attention.h.
 //
 // The n query tokens of a sequence and the G = H / KH query heads of a key / value head make n * G rows, row = token * G + head in the group:
-// a work-group takes 128 of them, so short prompts fill its tiles with heads, and the keys of a group are staged once for all of its heads.
-// Tiles are numbered without knowing a length on the host: sequence s starts at tile floor(cu_q[s] G / 128) + s, which leaves each at
-// least ceil(n G / 128) numbers; a work-group finds its sequence by a 64-ary search over cu_q and returns if its number is spare.
+// a work-group takes kRows of them, so short prompts fill its tiles with heads, and the keys of a group are staged once for all of its heads.
+// Tiles are numbered without knowing a length on the host: sequence s starts at tile floor(cu_q[s] G / kRows) + s, which leaves each at
+// least ceil(n G / kRows) numbers; a work-group finds its sequence by a 64-ary search over cu_q and returns if its number is spare.
 // Later tiles of a causal sequence see more keys and are launched first; the key / value head is the fastest index of the grid, so with 8 (or a
 // multiple or divisor of 8) of them a head's keys stay in the L2 of its XCDs.
 #include "tile_attention.h"
@@ -24,16 +24,15 @@ struct PromptK {
   float scale, sc;
 };
 
-constexpr int kRows = 128;
-
 __device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
   const int64_t v = cu[i];
   return v < 0 ? 0 : v > most ? most : v;
 }
 
 template <typename Tile>
-__global__ void __launch_bounds__(256) prompt_attention_kernel(const PromptK a) {
+__global__ void __launch_bounds__(256, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
   typedef typename Tile::type T;
+  constexpr int kRows = Tile::kRows, RB = Tile::RB;
   const int kh = (int)blockIdx.x % a.KH;
   const int64_t tile = a.ntiles - 1 - (int)blockIdx.x / a.KH;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
@@ -53,61 +52,75 @@ __global__ void __launch_bounds__(256) prompt_attention_kernel(const PromptK a) 
   const int64_t row0 = (tile - (q0 * a.G / kRows + s)) * kRows;
   if (row0 < 0 || row0 >= rows) return;
 
-  // ---- what this lane's row, its wave and the work-group see
-  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int64_t {
-    if (!a.causal) return m;
-    const int64_t c = row / a.G + 1 + m - n;
-    return c < 0 ? 0 : c > m ? m : c;
+  // ---- what the rows see
+  auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int {
+    const int64_t c = a.causal ? row / a.G + 1 + m - n : m;
+    return (int)(c < 0 ? 0 : c > m ? m : c);
   };
-  const int64_t last = rows - 1;
-  const int64_t wrow = row0 + 32 * wave, row = wrow + q32;
-  const bool live = row <= last;
-  const int64_t limit = live ? limit_of(row) : 0;
-  const int64_t wave_min = wrow <= last ? limit_of(wrow) : 0;
-  const int64_t wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
-  const int64_t nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
-
-  const int64_t token = q0 + (live ? row / a.G : 0);
-  const int head = kh * a.G + (live ? (int)(row % a.G) : 0);
+  const int64_t last = rows - 1, wrow = row0 + 32 * RB * wave;
+  AttnLimits<RB> lim;
+  lim.wave_min = wrow <= last ? limit_of(wrow) : 0;
+  lim.wave_max = wrow <= last ? limit_of(wrow + 32 * RB - 1 < last ? wrow + 32 * RB - 1 : last) : 0;
+  lim.group_min = limit_of(row0);
+  lim.nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
   Tile t;
   AttnState<Tile> st;
   t.init(PP_DYN_SMEM);
-  t.load_q(live ? (const T*)a.q + token * a.q_row + head * a.q_head : nullptr, a.D);
-  attend(t, st, (const T*)a.k + k0 * a.k_row + kh * a.k_head, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.k_row, a.v_row, nkeys, limit,
-         wave_min, wave_max, a.D, a.sc);
-  if (!live) return;
-  // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
-  const float inv = limit > 0 ? 1.f / st.l : 0.f;
-  T* dst = (T*)a.out + token * a.out_row + head * a.out_head;
 #pragma unroll
-  for (int db = 0; db < Tile::kDB; ++db)
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t row = wrow + 32 * rb + q32;
+    const bool live = row <= last;
+    lim.row[rb] = live ? limit_of(row) : 0;
+    t.load_q(rb, live ? (const T*)a.q + (q0 + row / a.G) * a.q_row + (kh * a.G + row % a.G) * a.q_head : nullptr, a.D);
+  }
+  attend(t, st, (const T*)a.k + k0 * a.k_row + kh * a.k_head, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.k_row, a.v_row, lim, a.D, a.sc);
+  if (st.not_finite) add_not_finite(t, st, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.v_row, lim, a.D);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * db + 8 * g + 4 * h;
-      if (d < a.D)
-        Tile::store4(dst + d, st.o[db][4 * g] * inv, st.o[db][4 * g + 1] * inv, st.o[db][4 * g + 2] * inv, st.o[db][4 * g + 3] * inv);
-    }
-  if (a.lse && h == 0) a.lse[token * a.H + head] = limit > 0 ? st.m * a.scale + logf(st.l) : neg_inf();
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t row = wrow + 32 * rb + q32;
+    if (row > last) continue;
+    const int64_t token = q0 + row / a.G;
+    const int head = kh * a.G + (int)(row % a.G);
+    // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
+    const float inv = lim.row[rb] > 0 ? 1.f / st.l[rb] : 0.f;
+    T* dst = (T*)a.out + token * a.out_row + head * a.out_head;
+#pragma unroll
+    for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * db + 8 * g + 4 * h;
+        const f16v& o = st.o[rb][db];
+        if (d < a.D) Tile::store4(dst + d, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
+      }
+    if (a.lse && h == 0) a.lse[token * a.H + head] = lim.row[rb] > 0 ? st.m[rb] * a.scale + logf(st.l[rb]) : neg_inf();
+  }
 }
 
 }  // namespace pp
 
-template <typename T, int DP>
-static int launch_prompt(void* stream, const pp::PromptK& a) {
+template <typename Tile>
+static int launch_prompt(void* stream, pp::PromptK& a) {
   using namespace pp;
-  typedef AttnTile<T, DP> Tile;
+  const int64_t ntiles = a.Tq * a.G / Tile::kRows + a.B;
+  if (ntiles * a.KH * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
+  a.ntiles = (int)ntiles;
   PP_ALLOW_BIG_LDS((&prompt_attention_kernel<Tile>), Tile::kSmem);
   PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH)), dim3(256), Tile::kSmem, stream, a);
   return pp_check_launch("pp_prompt_attention");
 }
 
 template <typename T>
-static int launch_prompt_d(void* stream, const pp::PromptK& a) {
-  if (a.D <= 32) return launch_prompt<T, 32>(stream, a);
-  if (a.D <= 64) return launch_prompt<T, 64>(stream, a);
-  if (a.D <= 96) return launch_prompt<T, 96>(stream, a);
-  if (a.D <= 128) return launch_prompt<T, 128>(stream, a);
-  return launch_prompt<T, 256>(stream, a);
+static int launch_prompt_d(void* stream, pp::PromptK& a) {
+  using namespace pp;
+  if constexpr (sizeof(T) == 2) {
+    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 2>>(stream, a);
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 2>>(stream, a);
+  }
+  if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 1>>(stream, a);
+  if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 1>>(stream, a);
+  if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 1, 1>>(stream, a);
+  if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 1, 1>>(stream, a);
+  return launch_prompt<AttnTile<T, 256, 1, 1>>(stream, a);
 }
 
 extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p) {
@@ -135,9 +148,6 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
   a.Tq = p->Tq; a.Tk = p->Tk;
   a.B = (int)p->B; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D; a.causal = p->causal != 0;
   a.scale = p->scale; a.sc = p->scale * kLog2e;
-  const int64_t ntiles = p->Tq * a.G / kRows + p->B;
-  if (ntiles * p->KH * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
-  a.ntiles = (int)ntiles;
   if (p->dtype == PP_F32) return launch_prompt_d<float>(stream, a);
   if (p->dtype == PP_F16) return launch_prompt_d<half_t>(stream, a);
   return launch_prompt_d<bf16_t>(stream, a);

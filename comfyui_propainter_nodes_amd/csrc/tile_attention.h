@@ -1,21 +1,26 @@
 // tile_attention.h -- one work-group's attention over a run of keys: the part that pp_prompt_attention and pp_prefix_attention share.
 //
-// A work-group of 4 waves takes 128 query rows, 32 per wave, of ONE key / value head (the query heads of a group are rows of the
-// same tile, so their keys are staged once).  Keys are walked in tiles through LDS:
+// A work-group of 4 waves takes 128 RB query rows, 32 RB per wave, of ONE key / value head (the query heads of a group are rows of the
+// same tile, so their keys are staged once).  Keys are walked in steps of 32 NS through LDS:
 //   S^T = K . Q^T     32x32 MFMA; lane l holds the scores of query l & 31 against keys (r & 3) + 8 (r >> 2) + 4 (l >> 5), r = 0..15
 //   online softmax    lane-local, one exchange between lanes l and l ^ 32; fp32 maxima, sums and accumulators
 //   O^T += V^T . P^T  the lane's own probabilities are the B operand, V^T fragments come out of LDS transposed (f16 / bf16:
 //                     ds_read_b64_tr_b16; f32: one value per lane)
+// Step i works on three key blocks at once -- the softmax of block i, the second product of block i - 1 and the first of block i + 1 -- so
+// every MFMA of a step is independent of its exponentials.  K and V pass through two LDS slots each; their loads are issued a step
+// before they are stored, one barrier a step.
 // The running maximum that the probabilities refer to moves only when a score of the wave passes it by more than kDefer in the
-// exponent of 2, so most tiles rescale nothing.  A probability is then at most 2^kDefer, far inside f16 and exact in relative terms.
+// exponent of 2, so most steps rescale nothing.  A probability is then at most 2^kDefer, far inside f16 and exact in relative terms.
 //
 // Rows that see different numbers of keys: `limit` is the row's own count, scores at or past it become -inf before the softmax.  Their
 // probability is 0, but 0 x V is NaN for a V that is not finite.  Keys past the last one that any row of the work-group sees are staged as
-// zeros; a sub-tile in which only some rows see a key whose V is not finite goes through pv_guarded(), which multiplies
-// the finite part and adds infinities and NaN to the rows that see them and to no others.
+// zeros; in blocks that only some rows see, V values that are not finite are staged as zeros too, and if there were any, add_not_finite()
+// goes over those blocks once more at the end and adds them to the rows that do see them.
 #pragma once
 #include "attn_device.h"
 #include "bf16_device.h"
+
+#include <type_traits>
 
 namespace pp {
 
@@ -33,13 +38,13 @@ template <typename T>
 struct Op;
 template <>
 struct Op<half_t> {
-  static constexpr unsigned kExp = 0x7c007c00u, kCarry = 0x04000400u, kOne = 0x3c00u;
+  static constexpr unsigned kExp = 0x7c007c00u, kCarry = 0x04000400u;
   static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return mfma_32x32x16_f16(a, b, c); }
   static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, h2{(half_t)a, (half_t)b}); }
 };
 template <>
 struct Op<bf16_t> {
-  static constexpr unsigned kExp = 0x7f807f80u, kCarry = 0x00800080u, kOne = 0x3f80u;
+  static constexpr unsigned kExp = 0x7f807f80u, kCarry = 0x00800080u;
 #ifndef PP_EMU
   typedef __bf16 hw8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) {
@@ -76,152 +81,109 @@ struct Op<bf16_t> {
 __device__ __forceinline__ int score_key(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
 // ----------------------------------------------------------------------------------------
-// 16-bit storage.  K and V tiles of kBN keys lie in LDS row by row, kPitch bytes a row, their 16-byte pieces XOR-swizzled so that the
-// K reads (16 bytes of 32 rows at once) and the transposing V reads (64 bytes of 4 rows at once) touch every bank once.
+// 16-bit storage.  The two K and two V slots of 32 NS keys lie in LDS row by row, kPitch bytes a row, their 16-byte pieces XOR-swizzled so
+// that the K reads (16 bytes of 32 rows at once) and the transposing V reads (64 bytes of 4 rows at once) touch every bank once.
 // ----------------------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, int RB_, int NS_>
 struct AttnTile {
   typedef T type;
-  static constexpr int kBN = DP > 128 ? 32 : 64;
+  static constexpr int RB = RB_, NS = NS_, kBN = 32 * NS, kRows = 128 * RB;
+  static constexpr int kWaves = RB > 1 || DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kPitch = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
-  static constexpr int kPieces = DP / 8, kStage = kBN * kPieces / 256, kDB = DP / 32, kQF = DP / 16;
-  static constexpr int kSmem = 2 * kBN * kPitch;
-  static_assert(kBN * kPieces % 256 == 0, "a tile is dealt to 256 threads");
+  static constexpr int kPieces = DP / 8, kPer = 8, kAll = kBN * kPieces, kStage = (kAll + 255) / 256, kDB = DP / 32, kQF = DP / 16;
+  static constexpr int kSlot = kBN * kPitch, kFlag = 4 * kSlot, kSmem = kFlag + 16;
+  struct P {
+    h8 f[2];
+  };
 
-  h8 q[kQF];
-  u4 ks[kStage], vs[kStage];  // the next tile on its way
+  h8 q[RB][kQF];
+  u4 ks[kStage], vs[kStage];  // blocks on their way
   unsigned char* smem;
   int q32, h;
 
-  static __device__ __forceinline__ int k_slot(int row, int piece) {
+  static __device__ __forceinline__ int k_at(int slot, int row, int piece) {
     constexpr int m = kPitch >= 256 ? 15 : kPitch / 16 - 1, sh = kPitch >= 256 ? 0 : kPitch == 128 ? 1 : 2;
-    return row * kPitch + ((piece ^ ((row >> sh) & m)) << 4);
+    return slot * kSlot + row * kPitch + ((piece ^ ((row >> sh) & m)) << 4);
   }
-  static __device__ __forceinline__ int v_slot(int row, int piece) {
+  static __device__ __forceinline__ int v_at(int slot, int row, int piece) {
     constexpr int m = kPitch >= 256 ? 3 : kPitch == 128 ? 1 : 0, sh = kPitch >= 256 ? 0 : 1;
-    return kBN * kPitch + row * kPitch + ((piece ^ (((row >> sh) & m) << 2)) << 4);
+    return (2 + slot) * kSlot + row * kPitch + ((piece ^ (((row >> sh) & m) << 2)) << 4);
   }
   __device__ __forceinline__ void init(unsigned char* lds) {
     smem = lds;
     q32 = (int)threadIdx.x & 31;
     h = ((int)threadIdx.x >> 5) & 1;
   }
-  // row: this lane's query, or null
-  __device__ __forceinline__ void load_q(const T* row, int D) {
+  // row: this lane's query of row block rb, or null
+  __device__ __forceinline__ void load_q(int rb, const T* row, int D) {
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
       const int d = 16 * c + 8 * h;
       u4 v = {0u, 0u, 0u, 0u};
       if (row && d < D) v = *reinterpret_cast<const u4*>(row + d);
-      q[c] = __builtin_bit_cast(h8, v);
+      q[rb][c] = __builtin_bit_cast(h8, v);
     }
   }
-  __device__ __forceinline__ void load_tile(const T* k, const T* v, int64_t k_row, int64_t v_row, int64_t kt, int64_t nkeys, int D) {
+  static __device__ __forceinline__ u4 load_piece(const T* src) { return *reinterpret_cast<const u4*>(src); }
+  __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + k_at(slot, row, piece)) = ks[i]; }
+  __device__ __forceinline__ void store_v(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + v_at(slot, row, piece)) = vs[i]; }
+  __device__ __forceinline__ void qk(int slot, f16v (*s)[NS]) const {
 #pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int at = (int)threadIdx.x + 256 * i, row = at / kPieces, piece = at - row * kPieces;
-      ks[i] = vs[i] = u4{0u, 0u, 0u, 0u};
-      if (kt + row < nkeys && 8 * piece < D) {
-        ks[i] = *reinterpret_cast<const u4*>(k + (kt + row) * k_row + 8 * piece);
-        vs[i] = *reinterpret_cast<const u4*>(v + (kt + row) * v_row + 8 * piece);
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rb][sub][r] = 0.f;
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+      for (int c = 0; c < kQF; ++c) {
+        const h8 a = *reinterpret_cast<const h8*>(smem + k_at(slot, 32 * sub + q32, 2 * c + h));
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) s[rb][sub] = Op<T>::mfma(a, q[rb][c], s[rb][sub]);
       }
-    }
   }
-  __device__ __forceinline__ void store_tile() {
-#pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int at = (int)threadIdx.x + 256 * i, row = at / kPieces, piece = at - row * kPieces;
-      *reinterpret_cast<u4*>(smem + k_slot(row, piece)) = ks[i];
-      *reinterpret_cast<u4*>(smem + v_slot(row, piece)) = vs[i];
-    }
-  }
-  __device__ __forceinline__ f16v qk(int sub) const {
-    f16v s;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-    for (int c = 0; c < kQF; ++c) {
-      const h8 a = *reinterpret_cast<const h8*>(smem + k_slot(32 * sub + q32, 2 * c + h));
-      s = Op<T>::mfma(a, q[c], s);
-    }
-    return s;
-  }
-  static __device__ __forceinline__ void pack_p(const float* p, h8* pf) {
+  static __device__ __forceinline__ P pack_p(const float* p) {
+    P f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       u4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = Op<T>::pack(p[8 * m + 2 * j], p[8 * m + 2 * j + 1]);
-      pf[m] = __builtin_bit_cast(h8, w);
+      f.f[m] = __builtin_bit_cast(h8, w);
     }
+    return f;
   }
   // V^T fragment of head-dim block db, 16-key group m of sub-tile `sub`: rows d = 32 db + (lane & 31), keys in score order
-  __device__ __forceinline__ h8 v_frag(int sub, int db, int m) const {
+  __device__ __forceinline__ h8 v_frag(int slot, int sub, int db, int m) const {
     const int lane = lane_id(), i = lane & 15, ir = i >> 2, g16 = lane >> 4;
     const int row = 32 * sub + 16 * m + 4 * h + ir, piece = 4 * db + 2 * (g16 & 1) + ((i & 3) >> 1);
-    const h4 lo = lds_read_tr16(reinterpret_cast<const half_t*>(smem + v_slot(row, piece) + (i & 1) * 8));
-    const h4 hi = lds_read_tr16(reinterpret_cast<const half_t*>(smem + v_slot(row + 8, piece) + (i & 1) * 8));
+    const h4 lo = lds_read_tr16(reinterpret_cast<const half_t*>(smem + v_at(slot, row, piece) + (i & 1) * 8));
+    const h4 hi = lds_read_tr16(reinterpret_cast<const half_t*>(smem + v_at(slot, row + 8, piece) + (i & 1) * 8));
     return h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
-  __device__ __forceinline__ void pv(int sub, const float* p, f16v* o) const {
-    h8 pf[2];
-    pack_p(p, pf);
+  __device__ __forceinline__ void pv(int slot, const P (*p)[NS], f16v (*o)[kDB]) const {
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) o[db] = Op<T>::mfma(v_frag(sub, db, m), pf[m], o[db]);
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) {
+          const h8 a = v_frag(slot, sub, db, m);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) o[rb][db] = Op<T>::mfma(a, p[rb][sub].f[m], o[rb][db]);
+        }
   }
-  // does the sub-tile's V hold a value that is not finite?  (exponent all ones: adding one to it carries out of the field)
-  __device__ __forceinline__ bool v_not_finite(int sub) const {
+  // zeroes what is not finite (exponent all ones: adding one to it carries out of the field); was there any?
+  static __device__ __forceinline__ bool scrub(u4& w) {
     unsigned any = 0;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        const u4 w = __builtin_bit_cast(u4, v_frag(sub, db, m));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) any |= ((w[j] & Op<T>::kExp) + Op<T>::kCarry) & 0x80008000u;
-      }
-    return wave_any(any != 0);
-  }
-  __device__ __forceinline__ void pv_guarded(int sub, const float* p, const bool* seen, f16v* o) const {
-    h8 pf[2], sf[2];
-    float sv[16];
-    pack_p(p, pf);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sv[r] = seen[r] ? 1.f : 0.f;
-    pack_p(sv, sf);
-#pragma unroll
-    for (int db = 0; db < kDB; ++db) {
-      f16v pos, neg, nan;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pos[r] = neg[r] = nan[r] = 0.f;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        u4 w = __builtin_bit_cast(u4, v_frag(sub, db, m)), wp = {0, 0, 0, 0}, wn = wp, wx = wp;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int s = 0; s < 32; s += 16) {
-            const unsigned x = (w[j] >> s) & 0xffffu, e = Op<T>::kExp & 0xffffu;
-            if ((x & e) != e) continue;
-            if (x & 0x7fffu & ~e) wx[j] |= Op<T>::kOne << s;
-            else if (x & 0x8000u) wn[j] |= Op<T>::kOne << s;
-            else wp[j] |= Op<T>::kOne << s;
-            w[j] &= ~(0xffffu << s);
-          }
-        o[db] = Op<T>::mfma(__builtin_bit_cast(h8, w), pf[m], o[db]);
-        pos = Op<T>::mfma(__builtin_bit_cast(h8, wp), sf[m], pos);
-        neg = Op<T>::mfma(__builtin_bit_cast(h8, wn), sf[m], neg);
-        nan = Op<T>::mfma(__builtin_bit_cast(h8, wx), sf[m], nan);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (pos[r] > 0.f) o[db][r] -= neg_inf();
-        if (neg[r] > 0.f) o[db][r] += neg_inf();
-        if (nan[r] > 0.f) o[db][r] = __builtin_nanf("");
-      }
+    for (int j = 0; j < 4; ++j) {
+      const unsigned bad = ((w[j] & Op<T>::kExp) + Op<T>::kCarry) & 0x80008000u;  // the top bit of each bad half
+      any |= bad;
+      w[j] &= ~((bad >> 15) * 0xffffu);
     }
+    return any != 0;
   }
   // 4 consecutive head-dim values of a row
   static __device__ __forceinline__ void store4(T* dst, float a, float b, float c, float d) {
@@ -233,16 +195,21 @@ struct AttnTile {
 // f32 storage: both products on v_mfma_f32_32x32x2_f32 (64 cycles for 2 keys or channels: the matrix pipe is the bound by far, LDS and
 // the vector ALU have slack).  Rows have a pitch of DP + 4 floats.
 // ----------------------------------------------------------------------------------------
-template <int DP>
-struct AttnTile<float, DP> {
+template <int DP, int RB_, int NS_>
+struct AttnTile<float, DP, RB_, NS_> {
   typedef float type;
-  static constexpr int kBN = 32;
+  static_assert(RB_ == 1 && NS_ == 1, "f32: one row block, 32 keys a step");
+  static constexpr int RB = 1, NS = 1, kBN = 32, kRows = 128;
+  static constexpr int kWaves = DP > 64 ? 1 : 2;  // per SIMD
   static constexpr int kP = DP + 4;
-  static constexpr int kPieces = DP / 4, kStage = kBN * kPieces / 256, kDB = DP / 32, kQF = DP / 8;
-  static constexpr int kSmem = 2 * kBN * kP * 4;
+  static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + 255) / 256, kDB = DP / 32, kQF = DP / 8;
+  static constexpr int kSlot = kBN * kP, kFlag = 4 * kSlot * 4, kSmem = kFlag + 16;
+  struct P {
+    float f[16];
+  };
 
-  f4 q[kQF];
-  f4 ks[kStage], vs[kStage];
+  f4 q[1][kQF];
+  u4 ks[kStage], vs[kStage];
   float* smem;
   int q32, h;
 
@@ -251,84 +218,54 @@ struct AttnTile<float, DP> {
     q32 = (int)threadIdx.x & 31;
     h = ((int)threadIdx.x >> 5) & 1;
   }
-  __device__ __forceinline__ void load_q(const float* row, int D) {
+  __device__ __forceinline__ void load_q(int, const float* row, int D) {
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
       const int d = 8 * c + 4 * h;
-      q[c] = f4{0.f, 0.f, 0.f, 0.f};
-      if (row && d < D) q[c] = *reinterpret_cast<const f4*>(row + d);
+      q[0][c] = f4{0.f, 0.f, 0.f, 0.f};
+      if (row && d < D) q[0][c] = *reinterpret_cast<const f4*>(row + d);
     }
   }
-  __device__ __forceinline__ void load_tile(const float* k, const float* v, int64_t k_row, int64_t v_row, int64_t kt, int64_t nkeys, int D) {
-#pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int at = (int)threadIdx.x + 256 * i, row = at / kPieces, piece = at - row * kPieces;
-      ks[i] = vs[i] = f4{0.f, 0.f, 0.f, 0.f};
-      if (kt + row < nkeys && 4 * piece < D) {
-        ks[i] = *reinterpret_cast<const f4*>(k + (kt + row) * k_row + 4 * piece);
-        vs[i] = *reinterpret_cast<const f4*>(v + (kt + row) * v_row + 4 * piece);
-      }
-    }
+  static __device__ __forceinline__ u4 load_piece(const float* src) { return *reinterpret_cast<const u4*>(src); }
+  __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const {
+    *reinterpret_cast<u4*>(smem + slot * kSlot + row * kP + 4 * piece) = ks[i];
   }
-  __device__ __forceinline__ void store_tile() {
-#pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int at = (int)threadIdx.x + 256 * i, row = at / kPieces, piece = at - row * kPieces;
-      *reinterpret_cast<f4*>(smem + row * kP + 4 * piece) = ks[i];
-      *reinterpret_cast<f4*>(smem + kBN * kP + row * kP + 4 * piece) = vs[i];
-    }
+  __device__ __forceinline__ void store_v(int slot, int i, int row, int piece) const {
+    *reinterpret_cast<u4*>(smem + (2 + slot) * kSlot + row * kP + 4 * piece) = vs[i];
   }
   // channels are taken in the order (8c + 4h + j): any order serves a dot product as long as both operands share it
-  __device__ __forceinline__ f16v qk(int) const {
-    f16v s;
+  __device__ __forceinline__ void qk(int slot, f16v (*s)[1]) const {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    for (int r = 0; r < 16; ++r) s[0][0][r] = 0.f;
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
-      const f4 a = *reinterpret_cast<const f4*>(smem + q32 * kP + 8 * c + 4 * h);
+      const f4 a = *reinterpret_cast<const f4*>(smem + slot * kSlot + q32 * kP + 8 * c + 4 * h);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s = mfma_32x32x2_f32(a[j], q[c][j], s);
+      for (int j = 0; j < 4; ++j) s[0][0] = mfma_32x32x2_f32(a[j], q[0][c][j], s[0][0]);
     }
-    return s;
   }
-  __device__ __forceinline__ float v_at(int r, int db) const { return smem[kBN * kP + score_key(r, h) * kP + 32 * db + q32]; }
-  __device__ __forceinline__ void pv(int, const float* p, f16v* o) const {
+  static __device__ __forceinline__ P pack_p(const float* p) {
+    P f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f.f[r] = p[r];
+    return f;
+  }
+  __device__ __forceinline__ float v_val(int slot, int r, int db) const { return smem[(2 + slot) * kSlot + score_key(r, h) * kP + 32 * db + q32]; }
+  __device__ __forceinline__ void pv(int slot, const P (*p)[1], f16v (*o)[kDB]) const {
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) o[db] = mfma_32x32x2_f32(v_at(r, db), p[r], o[db]);
+      for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
   }
-  __device__ __forceinline__ bool v_not_finite(int) const {
+  static __device__ __forceinline__ bool scrub(u4& w) {
     bool any = false;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) any |= (__builtin_bit_cast(unsigned, v_at(r, db)) & 0x7f800000u) == 0x7f800000u;
-    return wave_any(any);
-  }
-  __device__ __forceinline__ void pv_guarded(int, const float* p, const bool* seen, f16v* o) const {
-#pragma unroll
-    for (int db = 0; db < kDB; ++db) {
-      f16v pos, neg, nan;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pos[r] = neg[r] = nan[r] = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float v = v_at(r, db), w = seen[r] ? 1.f : 0.f;
-        const unsigned u = __builtin_bit_cast(unsigned, v);
-        const bool bad = (u & 0x7f800000u) == 0x7f800000u, isnan = bad && (u & 0x7fffffu);
-        o[db] = mfma_32x32x2_f32(bad ? 0.f : v, p[r], o[db]);
-        pos = mfma_32x32x2_f32(bad && !isnan && !(u >> 31) ? 1.f : 0.f, w, pos);
-        neg = mfma_32x32x2_f32(bad && !isnan && (u >> 31) ? 1.f : 0.f, w, neg);
-        nan = mfma_32x32x2_f32(isnan ? 1.f : 0.f, w, nan);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (pos[r] > 0.f) o[db][r] -= neg_inf();
-        if (neg[r] > 0.f) o[db][r] += neg_inf();
-        if (nan[r] > 0.f) o[db][r] = __builtin_nanf("");
-      }
+    for (int j = 0; j < 4; ++j) {
+      const bool bad = (w[j] & 0x7f800000u) == 0x7f800000u;
+      any |= bad;
+      w[j] = bad ? 0u : w[j];
     }
+    return any;
   }
   static __device__ __forceinline__ void store4(float* dst, float a, float b, float c, float d) {
     *reinterpret_cast<f4*>(dst) = f4{a, b, c, d};
@@ -340,74 +277,225 @@ struct AttnTile<float, DP> {
 // ----------------------------------------------------------------------------------------
 template <typename Tile>
 struct AttnState {
-  f16v o[Tile::kDB];  // O^T: row d = 32 db + score_key(r, h), column = the lane's query
-  float m, l;         // running maximum (of the raw scores; -inf before the first visible key) and this lane's part of the sum
+  f16v o[Tile::RB][Tile::kDB];     // O^T: row d = 32 db + score_key(r, h), column = the lane's query
+  float m[Tile::RB], l[Tile::RB];  // running maximum (of the raw scores; -inf before the first visible key) and the sum
+  bool not_finite;                 // values of V were left out: add_not_finite()
 };
 
-// Keys [0, nkeys) at k, v.  limit: keys that this lane's row sees (<= nkeys).  wave_min / wave_max: the smallest and largest limit among
-// the wave's live rows (wave-uniform; wave_max = 0: no live row, the wave only helps staging).  sc = scale * log2(e) > 0.
+// What the rows of a work-group see of its nkeys keys: this lane's rows, the smallest / largest count among the wave's live rows (both 0
+// without one) and the smallest among the work-group's.
+template <int RB>
+struct AttnLimits {
+  int row[RB], wave_min, wave_max, group_min, nkeys;
+};
+
+// k, v: the first key.  sc = scale * log2(e) > 0.
 template <typename Tile>
 __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typename Tile::type* k, const typename Tile::type* v,
-                                       int64_t k_row, int64_t v_row, int64_t nkeys, int64_t limit, int64_t wave_min, int64_t wave_max,
-                                       int D, float sc) {
+                                       int64_t k_row, int64_t v_row, const AttnLimits<Tile::RB>& lim, int D, float sc) {
+  typedef typename Tile::type T;
+  typedef typename Tile::P P;
+  constexpr int RB = Tile::RB, NS = Tile::NS, BN = Tile::kBN;
 #pragma unroll
-  for (int db = 0; db < Tile::kDB; ++db)
+  for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) st.o[db][r] = 0.f;
-  st.m = neg_inf();
-  st.l = 0.f;
-  if (nkeys <= 0) return;
-  t.load_tile(k, v, k_row, v_row, 0, nkeys, D);
-  for (int64_t kt = 0; kt < nkeys; kt += Tile::kBN) {
-    t.store_tile();
-    __syncthreads();
-    if (kt + Tile::kBN < nkeys) t.load_tile(k, v, k_row, v_row, kt + Tile::kBN, nkeys, D);
+    for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
-    for (int sub = 0; sub < Tile::kBN / 32; ++sub) {
-      const int64_t k0 = kt + 32 * sub;
-      if (k0 >= wave_max) break;
-      f16v s = t.qk(sub);
-      const bool masked = k0 + 32 > wave_min;
-      const int left = (int)(limit - k0 < 32 ? limit - k0 : 32);  // keys of this sub-tile that the row sees (may be negative)
-      if (masked) {
+      for (int r = 0; r < 16; ++r) st.o[rb][db][r] = 0.f;
+    st.m[rb] = neg_inf();
+    st.l[rb] = 0.f;
+  }
+  st.not_finite = false;
+  const int nsteps = (lim.nkeys + BN - 1) / BN;
+  if (nsteps <= 0) return;
+
+  // ---- staging: thread -> (row, 16-byte piece) of a block
+  int prow[Tile::kStage], ppiece[Tile::kStage];
+  int64_t koff[Tile::kStage], voff[Tile::kStage];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = score_key(r, t.h) < left ? s[r] : neg_inf();
+  for (int i = 0; i < Tile::kStage; ++i) {
+    const int at = (int)threadIdx.x + 256 * i;
+    prow[i] = at / Tile::kPieces;
+    ppiece[i] = at - prow[i] * Tile::kPieces;
+    koff[i] = prow[i] * k_row + ppiece[i] * Tile::kPer;
+    voff[i] = prow[i] * v_row + ppiece[i] * Tile::kPer;
+    if (ppiece[i] * Tile::kPer >= D) prow[i] = 1 << 30;  // a piece past the head dim is zeros
+  }
+  const int mixed_from = lim.group_min;  // from this key on some rows see what others do not
+  volatile int* const flag = reinterpret_cast<volatile int*>(reinterpret_cast<unsigned char*>(t.smem) + Tile::kFlag);
+  if (threadIdx.x == 0) *flag = 0;
+  const T* const zero = reinterpret_cast<const T*>(pp_zero16);
+  auto load_k = [&](u4* dst, int i) __attribute__((always_inline)) {
+    const T* base = k + (int64_t)i * BN * k_row;
+    const int left = lim.nkeys - i * BN;
+#pragma unroll
+    for (int j = 0; j < Tile::kStage; ++j) dst[j] = Tile::load_piece(prow[j] < left ? base + koff[j] : zero);
+  };
+  auto load_v = [&](int i) __attribute__((always_inline)) {
+    const T* base = v + (int64_t)i * BN * v_row;
+    const int left = lim.nkeys - i * BN;
+#pragma unroll
+    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = Tile::load_piece(prow[j] < left ? base + voff[j] : zero);
+  };
+  auto store_k = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < Tile::kStage; ++j) {
+      const int at = (int)threadIdx.x + 256 * j, row = at / Tile::kPieces;
+      if (Tile::kAll % 256 == 0 || at < Tile::kAll) t.store_k(slot, j, row, at - row * Tile::kPieces);
+    }
+  };
+  auto store_v = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < Tile::kStage; ++j) {
+      const int at = (int)threadIdx.x + 256 * j, row = at / Tile::kPieces;
+      if (Tile::kAll % 256 == 0 || at < Tile::kAll) t.store_v(slot, j, row, at - row * Tile::kPieces);
+    }
+  };
+
+  f16v s[RB][NS];  // scores of the block whose softmax is next
+  P p[RB][NS];     // probabilities of the block before it
+  // softmax of block i, second product of block i - 1, first product of block i + 1; fast: every live row of the work-group sees all of it
+  auto step = [&](int i, int s0, auto fast) __attribute__((always_inline)) {
+    constexpr bool kFast = decltype(fast)::value;
+    const int s1 = 1 - s0;
+    store_k(s0);  // block i + 2
+    if (!kFast && mixed_from < lim.nkeys && (i + 1) * BN > mixed_from) {
+#pragma unroll
+      for (int j = 0; j < Tile::kStage; ++j)
+        if (Tile::scrub(t.vs[j])) *flag = 1;
+    }
+    store_v(s0);  // block i
+    load_k(t.ks, i + 3);
+    load_v(i + 1);
+    if (kFast ? lim.wave_max > 0 : i * BN < lim.wave_max) {
+      if constexpr (!kFast) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int sub = 0; sub < NS; ++sub) {
+            const int left = lim.row[rb] - i * BN - 32 * sub;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
+          }
       }
-      float mt = s[0];
+      float mt[RB], alpha[RB], nm[RB];
+      bool moved = false;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-      mt = fmaxf(st.m, pair32_max(mt));
-      // (-inf) - (-inf) is NaN and compares false: a row that has seen nothing yet moves nothing
-      if (wave_any((mt - st.m) * sc > kDefer)) {
-        const float alpha = mt == st.m ? 1.f : fast_exp2((st.m - mt) * sc);
-        st.l *= alpha;
+      for (int rb = 0; rb < RB; ++rb) {
+        float x = s[rb][0][0];
 #pragma unroll
-        for (int db = 0; db < Tile::kDB; ++db)
+        for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) st.o[db][r] *= alpha;
-        st.m = mt;
+          for (int r = 0; r < 16; ++r) x = fmaxf(x, s[rb][sub][r]);
+        mt[rb] = fmaxf(st.m[rb], pair32_max(x));
+        // (-inf) - (-inf) is NaN and compares false: a row that has seen nothing yet moves nothing
+        moved |= (mt[rb] - st.m[rb]) * sc > kDefer;
       }
-      const float nm = st.m == neg_inf() ? 0.f : -st.m * sc;
-      float p[16];
+      const bool rescale = wave_any(moved);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        alpha[rb] = 1.f;
+        if (rescale) {
+          alpha[rb] = mt[rb] == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - mt[rb]) * sc);
+          st.l[rb] *= alpha[rb];
+          st.m[rb] = mt[rb];
+        }
+        nm[rb] = st.m[rb] == neg_inf() ? 0.f : -st.m[rb] * sc;
+      }
+      // ---- independent of each other: probabilities of i, second product of i - 1 (against the maximum as it was), first of i + 1
+      P pn[RB][NS];
+      f16v sn[RB][NS];
+      if (kFast || (i + 1) * BN < lim.wave_max) t.qk(s1, sn);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub) {
+          float e[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            e[r] = fast_exp2(__builtin_fmaf(s[rb][sub][r], sc, nm[rb]));
+            st.l[rb] += e[r];
+          }
+          pn[rb][sub] = Tile::pack_p(e);
+        }
+      if constexpr (kFast) t.pv(s1, p, st.o);
+      else if (i > 0) t.pv(s1, p, st.o);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub) {
+          p[rb][sub] = pn[rb][sub];
+          s[rb][sub] = sn[rb][sub];
+        }
+      if (rescale) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha[rb];
+      }
+    } else if (!kFast && i > 0 && (i - 1) * BN < lim.wave_max) {
+      t.pv(s1, p, st.o);
+    }
+    pp_barrier();
+  };
+
+  // ---- before step 0: K of blocks 0 and 1 in LDS, block 2 and V of block 0 on their way, scores of block 0
+  u4 k1[Tile::kStage];
+  load_k(t.ks, 0);
+  load_k(k1, 1);
+  load_v(0);
+  store_k(0);
+  load_k(t.ks, 2);
+#pragma unroll
+  for (int j = 0; j < Tile::kStage; ++j) {
+    const u4 two = t.ks[j];
+    t.ks[j] = k1[j];
+    k1[j] = two;
+  }
+  store_k(1);
+#pragma unroll
+  for (int j = 0; j < Tile::kStage; ++j) t.ks[j] = k1[j];
+  pp_barrier();
+  t.qk(0, s);
+  pp_barrier();
+  const int nfast = mixed_from / BN;
+  for (int i = 0; i < nsteps;) {
+    step(i, i & 1, std::false_type{});
+    if (++i == 1)
+      for (; i + 2 <= nfast; i += 2) {
+        step(i, 1, std::true_type{});
+        step(i + 1, 0, std::true_type{});
+      }
+  }
+  if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o);
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) st.l[rb] = pair32_sum(st.l[rb]);
+  st.not_finite = *flag != 0;
+}
+
+// Adds to o (weighted sums, normalised or not) what attend() left out: infinities and NaN of the keys that a row sees, from the first block
+// with a key that not every row of the work-group sees.
+template <typename Tile>
+__device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& st, const typename Tile::type* v, int64_t v_row,
+                                               const AttnLimits<Tile::RB>& lim, int D) {
+#pragma unroll 1
+  for (int key = lim.group_min / Tile::kBN * Tile::kBN; key < lim.nkeys; ++key) {
+    const typename Tile::type* row = v + key * v_row;
+#pragma unroll
+    for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = fast_exp2(__builtin_fmaf(s[r], sc, nm));
-        st.l += p[r];
-      }
-      bool guarded = false;
-      if (masked && wave_min < (nkeys < k0 + 32 ? nkeys : k0 + 32)) guarded = t.v_not_finite(sub);
-      if (guarded) {
-        bool seen[16];
+        const int d = 32 * db + score_key(r, t.h);
+        const float x = d < D ? to_f32(row[d]) : 0.f;
+        if ((__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) seen[r] = score_key(r, t.h) < left;
-        t.pv_guarded(sub, p, seen, st.o);
-      } else {
-        t.pv(sub, p, st.o);
+          for (int rb = 0; rb < Tile::RB; ++rb)
+            if (key < lim.row[rb]) st.o[rb][db][r] += x;
+        }
       }
-    }
-    __syncthreads();
   }
-  st.l = pair32_sum(st.l);
 }
 
 }  // namespace pp
