@@ -33,6 +33,30 @@ inline float neg_inf() { return -INFINITY; }
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 #endif
 
+#ifdef PP_EMU
+inline int opaque_uniform(int v) { return v; }
+inline void keep_branch() {}
+inline void pin(float&) {}
+inline void pin(unsigned&) {}
+#else
+__device__ __forceinline__ int opaque_uniform(int v) {
+  v = __builtin_amdgcn_readfirstlane(v);
+  asm volatile("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }  // the value is computed by here
+__device__ __forceinline__ void pin(unsigned& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }  // what follows is not computed ahead of its condition
+#endif
+// 16 bytes of global memory (a pointer that may be pp_zero16's would otherwise become a flat access, which counts as an LDS one too)
+__device__ __forceinline__ u4 load_global16(const void* src) {
+#ifdef PP_EMU
+  return *static_cast<const u4*>(src);
+#else
+  return *(const __attribute__((address_space(1))) u4*)src;
+#endif
+}
+
 // 16-bit operand types travel as h8 bit patterns
 template <typename T>
 struct Op;
@@ -124,7 +148,6 @@ struct AttnTile {
       q[rb][c] = __builtin_bit_cast(h8, v);
     }
   }
-  static __device__ __forceinline__ u4 load_piece(const T* src) { return *reinterpret_cast<const u4*>(src); }
   __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + k_at(slot, row, piece)) = ks[i]; }
   __device__ __forceinline__ void store_v(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + v_at(slot, row, piece)) = vs[i]; }
   __device__ __forceinline__ void qk(int slot, f16v (*s)[NS]) const {
@@ -173,6 +196,74 @@ struct AttnTile {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) o[rb][db] = Op<T>::mfma(a, p[rb][sub].f[m], o[rb][db]);
         }
+  }
+  // A whole step: w = K Q^T, o += V^T z, y = exp2(x sc + nm) with its sums added to l, mx = row maxima of w.  The MFMAs are laid out one
+  // fragment at a time, each followed by its share of the exponentials (and, once w is complete, of the maxima), and the
+  // LDS reads run kAhead fragments ahead: left to itself the compiler puts all the vector work behind the last MFMA, and waits for each read.
+  __device__ __forceinline__ void products(int slot, f16v (&w)[RB][NS], const P (&z)[RB][NS], f16v (*o)[kDB], const f16v (&x)[RB][NS],
+                                           P (&y)[RB][NS], const float* nm, float sc, float* l, float* mx) const {
+    constexpr int n1 = NS * kQF, n2 = NS * 2 * kDB, n = n1 + n2, kAhead = 3, kRing = kAhead + 1;
+    constexpr int kEl = RB * NS * 16;
+    h8 ring[kRing];
+    auto fragment = [&](int j) __attribute__((always_inline)) -> h8 {
+      if (j < n1) return *reinterpret_cast<const h8*>(smem + k_at(slot, 32 * (j / kQF) + q32, 2 * (j % kQF) + h));
+      const int i = j - n1;
+      return v_frag(slot, i / (2 * kDB), i % kDB, i / kDB % 2);
+    };
+    u4 yw[RB][NS][2];
+    float even = 0.f, top[RB];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) ring[j] = fragment(j);
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      if (j + kAhead < n) ring[(j + kAhead) % kRing] = fragment(j + kAhead);
+      const h8 a = ring[j % kRing];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        if (j < n1) {
+          const f16v zero = {};
+          w[rb][j / kQF] = Op<T>::mfma(a, q[rb][j % kQF], j % kQF == 0 ? zero : w[rb][j / kQF]);
+        } else {
+          const int i = j - n1;
+          o[rb][i % kDB] = Op<T>::mfma(a, z[rb][i / (2 * kDB)].f[i / kDB % 2], o[rb][i % kDB]);
+        }
+      }
+#pragma unroll
+      for (int e = kEl * j / n; e < kEl * (j + 1) / n; ++e) {
+        const int rb = e / (16 * NS), sub = e / 16 % NS, r = e % 16;
+        const float v = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+        l[rb] += v;
+        pin(l[rb]);
+        if (r % 2) {
+          unsigned two = Op<T>::pack(even, v);
+          pin(two);
+          yw[rb][sub][r / 8][r % 8 / 2] = two;
+        } else {
+          even = v;
+        }
+      }
+      if (j > n1) {
+#pragma unroll
+        for (int e = kEl * (j - n1 - 1) / (n2 - 1); e < kEl * (j - n1) / (n2 - 1); ++e) {
+          const int rb = e / (16 * NS), i = e % (16 * NS);
+          top[rb] = i == 0 ? w[rb][0][0] : fmaxf(top[rb], w[rb][i / 16][i % 16]);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          if (kEl * (j - n1) / (n2 - 1) > rb * 16 * NS) pin(top[rb]);
+      }
+      pp_sched_fence();
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      mx[rb] = pair32_max(top[rb]);
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          y[rb][sub].f[m] = __builtin_bit_cast(h8, yw[rb][sub][m]);
+        }
+    }
   }
   // zeroes what is not finite (exponent all ones: adding one to it carries out of the field); was there any?
   static __device__ __forceinline__ bool scrub(u4& w) {
@@ -226,7 +317,6 @@ struct AttnTile<float, DP, RB_, NS_> {
       if (row && d < D) q[0][c] = *reinterpret_cast<const f4*>(row + d);
     }
   }
-  static __device__ __forceinline__ u4 load_piece(const float* src) { return *reinterpret_cast<const u4*>(src); }
   __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const {
     *reinterpret_cast<u4*>(smem + slot * kSlot + row * kP + 4 * piece) = ks[i];
   }
@@ -256,6 +346,19 @@ struct AttnTile<float, DP, RB_, NS_> {
     for (int r = 0; r < 16; ++r)
 #pragma unroll
       for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
+  }
+  __device__ __forceinline__ void products(int slot, f16v (&w)[1][1], const P (&z)[1][1], f16v (*o)[kDB], const f16v (&x)[1][1],
+                                           P (&y)[1][1], const float* nm, float sc, float* l, float* mx) const {
+    qk(slot, w);
+    float top = w[0][0][0];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      y[0][0].f[r] = fast_exp2(__builtin_fmaf(x[0][0][r], sc, nm[0]));
+      l[0] += y[0][0].f[r];
+      top = fmaxf(top, w[0][0][r]);
+    }
+    pv(slot, z, o);
+    mx[0] = pair32_max(top);
   }
   static __device__ __forceinline__ bool scrub(u4& w) {
     bool any = false;
@@ -329,13 +432,13 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     const T* base = k + (int64_t)i * BN * k_row;
     const int left = lim.nkeys - i * BN;
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) dst[j] = Tile::load_piece(prow[j] < left ? base + koff[j] : zero);
+    for (int j = 0; j < Tile::kStage; ++j) dst[j] = load_global16(prow[j] < left ? base + koff[j] : zero);
   };
   auto load_v = [&](int i) __attribute__((always_inline)) {
     const T* base = v + (int64_t)i * BN * v_row;
     const int left = lim.nkeys - i * BN;
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = Tile::load_piece(prow[j] < left ? base + voff[j] : zero);
+    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = load_global16(prow[j] < left ? base + voff[j] : zero);
   };
   auto store_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -352,91 +455,107 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     }
   };
 
-  f16v s[RB][NS];  // scores of the block whose softmax is next
-  P p[RB][NS];     // probabilities of the block before it
-  // softmax of block i, second product of block i - 1, first product of block i + 1; fast: every live row of the work-group sees all of it
-  auto step = [&](int i, int s0, auto fast) __attribute__((always_inline)) {
-    constexpr bool kFast = decltype(fast)::value;
-    const int s1 = 1 - s0;
-    store_k(s0);  // block i + 2
-    if (!kFast && mixed_from < lim.nkeys && (i + 1) * BN > mixed_from) {
+  typedef f16v Scores[RB][NS];
+  typedef P Probs[RB][NS];
+  // scores of the block whose softmax is next, and their largest per row; probabilities of the block before it.  The second pair takes
+  // turns in the fast steps, so that nothing is copied.
+  Scores s, s2;
+  Probs p, p2;
+  float mx[RB];
+  auto block_max = [&](const Scores& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      float y = x[rb][0][0];
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y = fmaxf(y, x[rb][sub][r]);
+      mx[rb] = pair32_max(y);
+    }
+  };
+  float alpha[RB], nm[RB];
+  // the maximum moves if a row's passed it by more than kDefer; what was summed up to here is rescaled behind the block's products
+  auto move_max = [&]() __attribute__((always_inline)) -> int {
+    bool moved = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) moved |= (mx[rb] - st.m[rb]) * sc > kDefer;  // (-inf) - (-inf) is NaN: moves nothing
+    const int any = wave_any(moved);
+    if (any) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const float mt = fmaxf(st.m[rb], mx[rb]);
+        alpha[rb] = mt == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - mt) * sc);
+        st.l[rb] *= alpha[rb];
+        st.m[rb] = mt;
+        nm[rb] = mt == neg_inf() ? 0.f : -mt * sc;
+      }
+    }
+    return opaque_uniform(any);  // (or the compiler would make two copies of the block's products)
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {
+    keep_branch();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha[rb];
+  };
+  auto softmax = [&](const Scores& x, Probs& to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) {
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+          st.l[rb] += e[r];
+        }
+        to[rb][sub] = Tile::pack_p(e);
+      }
+  };
+  auto stage = [&](int i, int slot) __attribute__((always_inline)) {
+    store_k(slot);  // block i + 2
+    store_v(slot);  // block i
+    load_k(t.ks, i + 3);
+    load_v(i + 1);
+  };
+  // softmax of block i (x -> y), second product of block i - 1 (z), first product of block i + 1 (-> w); every live row of the work-group
+  // sees all of block i
+  auto fast_step = [&](int i, auto slot, const Scores& x, Scores& w, const Probs& z, Probs& y) __attribute__((always_inline)) {
+    constexpr int S0 = decltype(slot)::value, S1 = 1 - S0;
+    stage(i, S0);
+    if (lim.wave_max > 0) {
+      const int moved = move_max();
+      t.products(S1, w, z, st.o, x, y, nm, sc, st.l, mx);
+      if (moved) rescale();
+    }
+    pp_barrier();
+  };
+  // the same for any block: rows that see a part of it, waves that see none of it, no block before or behind it
+  auto any_step = [&](int i) __attribute__((always_inline)) {
+    const int s0 = i & 1, s1 = 1 - s0;
+    if (mixed_from < lim.nkeys && (i + 1) * BN > mixed_from) {
 #pragma unroll
       for (int j = 0; j < Tile::kStage; ++j)
         if (Tile::scrub(t.vs[j])) *flag = 1;
     }
-    store_v(s0);  // block i
-    load_k(t.ks, i + 3);
-    load_v(i + 1);
-    if (kFast ? lim.wave_max > 0 : i * BN < lim.wave_max) {
-      if constexpr (!kFast) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int sub = 0; sub < NS; ++sub) {
-            const int left = lim.row[rb] - i * BN - 32 * sub;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
-          }
-      }
-      float mt[RB], alpha[RB], nm[RB];
-      bool moved = false;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float x = s[rb][0][0];
-#pragma unroll
-        for (int sub = 0; sub < NS; ++sub)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x = fmaxf(x, s[rb][sub][r]);
-        mt[rb] = fmaxf(st.m[rb], pair32_max(x));
-        // (-inf) - (-inf) is NaN and compares false: a row that has seen nothing yet moves nothing
-        moved |= (mt[rb] - st.m[rb]) * sc > kDefer;
-      }
-      const bool rescale = wave_any(moved);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        alpha[rb] = 1.f;
-        if (rescale) {
-          alpha[rb] = mt[rb] == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - mt[rb]) * sc);
-          st.l[rb] *= alpha[rb];
-          st.m[rb] = mt[rb];
-        }
-        nm[rb] = st.m[rb] == neg_inf() ? 0.f : -st.m[rb] * sc;
-      }
-      // ---- independent of each other: probabilities of i, second product of i - 1 (against the maximum as it was), first of i + 1
-      P pn[RB][NS];
-      f16v sn[RB][NS];
-      if (kFast || (i + 1) * BN < lim.wave_max) t.qk(s1, sn);
+    stage(i, s0);
+    if (i > 0 && (i - 1) * BN < lim.wave_max) t.pv(s1, p, st.o);
+    if (i * BN < lim.wave_max) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int sub = 0; sub < NS; ++sub) {
-          float e[16];
+          const int left = lim.row[rb] - i * BN - 32 * sub;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            e[r] = fast_exp2(__builtin_fmaf(s[rb][sub][r], sc, nm[rb]));
-            st.l[rb] += e[r];
-          }
-          pn[rb][sub] = Tile::pack_p(e);
+          for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
         }
-      if constexpr (kFast) t.pv(s1, p, st.o);
-      else if (i > 0) t.pv(s1, p, st.o);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int sub = 0; sub < NS; ++sub) {
-          p[rb][sub] = pn[rb][sub];
-          s[rb][sub] = sn[rb][sub];
-        }
-      if (rescale) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int db = 0; db < Tile::kDB; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha[rb];
-      }
-    } else if (!kFast && i > 0 && (i - 1) * BN < lim.wave_max) {
-      t.pv(s1, p, st.o);
+      block_max(s);
+      if (move_max()) rescale();
+      softmax(s, p);
+      if ((i + 1) * BN < lim.wave_max) t.qk(s1, s);
     }
     pp_barrier();
   };
@@ -461,13 +580,17 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   t.qk(0, s);
   pp_barrier();
   const int nfast = mixed_from / BN;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) alpha[rb] = 1.f, nm[rb] = 0.f;
   for (int i = 0; i < nsteps;) {
-    step(i, i & 1, std::false_type{});
-    if (++i == 1)
+    any_step(i);
+    if (++i == 1 && i + 2 <= nfast) {
+      block_max(s);
       for (; i + 2 <= nfast; i += 2) {
-        step(i, 1, std::true_type{});
-        step(i + 1, 0, std::true_type{});
+        fast_step(i, std::integral_constant<int, 1>{}, s, s2, p, p2);
+        fast_step(i + 1, std::integral_constant<int, 0>{}, s2, s, p2, p);
       }
+    }
   }
   if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o);
 #pragma unroll
