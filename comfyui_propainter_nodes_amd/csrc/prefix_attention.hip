@@ -10,6 +10,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 namespace pp {
 
 struct PrefixK {
@@ -168,11 +170,19 @@ static int launch_prefix_d(void* stream, pp::PrefixK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
     if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 2>>(stream, a);
+#ifdef RB2
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 2, 2>>(stream, a);
+#elif defined(NS1)
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 1>>(stream, a);
+#endif
     if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 2>>(stream, a);
   }
   if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 1>>(stream, a);
   if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 1>>(stream, a);
   if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 1, 1>>(stream, a);
+#ifdef RB2
+  if constexpr (sizeof(T) == 2) if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 2, 1>>(stream, a);
+#endif
   if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 1, 1>>(stream, a);
   return launch_prefix<AttnTile<T, 256, 1, 1>>(stream, a);
 }
@@ -196,6 +206,9 @@ extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_p
                                p->ko_row, p->ko_head, p->vo_seq, p->vo_row, p->vo_head, p->out_seq, p->out_row, p->out_head};
   for (int i = 0; i < 16; ++i)
     if (strides[i] < 0 || strides[i] % e) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: strides must be >= 0 and keep rows 16-byte aligned");
+  // (a block of keys is addressed with 32-bit byte offsets)
+  for (const int64_t row : {p->kp_row, p->vp_row, p->ko_row, p->vo_row})
+    if (row >= 1 << 24) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: a key or value row stride must be below 2^24 elements");
   if (((uintptr_t)p->q | (uintptr_t)p->kp | (uintptr_t)p->vp | (uintptr_t)p->ko | (uintptr_t)p->vo | (uintptr_t)p->out | (uintptr_t)p->scratch) % 16)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: tensors must be 16-byte aligned");
   if (p->B == 0 || p->L == 0) return PP_OK;  // no row to write

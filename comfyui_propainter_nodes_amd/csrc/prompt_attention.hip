@@ -12,6 +12,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 namespace pp {
 
 struct PromptK {
@@ -114,11 +116,19 @@ static int launch_prompt_d(void* stream, pp::PromptK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
     if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 2>>(stream, a);
+#ifdef RB2
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 2>>(stream, a);
+#elif defined(NS1)
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 1>>(stream, a);
+#endif
     if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 2>>(stream, a);
   }
   if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 1>>(stream, a);
   if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 1>>(stream, a);
   if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 1, 1>>(stream, a);
+#ifdef RB2
+  if constexpr (sizeof(T) == 2) if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 2, 1>>(stream, a);
+#endif
   if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 1, 1>>(stream, a);
   return launch_prompt<AttnTile<T, 256, 1, 1>>(stream, a);
 }
@@ -137,6 +147,9 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
   const int64_t strides[8] = {p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head, p->out_row, p->out_head};
   for (int i = 0; i < 8; ++i)
     if (strides[i] < 0 || strides[i] % e) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: strides must be >= 0 and keep rows 16-byte aligned");
+  // (a block of keys is addressed with 32-bit byte offsets)
+  for (const int64_t row : {p->k_row, p->v_row})
+    if (row >= 1 << 24) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: a key or value row stride must be below 2^24 elements");
   if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) % 16)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: tensors must be 16-byte aligned");
   if (p->B == 0 || p->Tq == 0) return PP_OK;  // no row to write

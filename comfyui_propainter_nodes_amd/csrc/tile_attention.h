@@ -9,8 +9,10 @@
 // Step i works on three key blocks at once -- the softmax of block i, the second product of block i - 1 and the first of block i + 1 -- so
 // every MFMA of a step is independent of its exponentials.  K and V pass through two LDS slots each; their loads are issued a step
 // before they are stored, one barrier a step.
-// The running maximum that the probabilities refer to moves only when a score of the wave passes it by more than kDefer in the
-// exponent of 2, so most steps rescale nothing.  A probability is then at most 2^kDefer, far inside f16 and exact in relative terms.
+// The maximum m that the probabilities 2^(s sc - m sc) refer to is a true one, but not the newest: a block is taken against the m it
+// finds, and only if a lane's sum over the block comes out above kMost (any probability would be then, or NaN) is m moved, what was summed
+// up rescaled and the block taken again.  No maximum is computed otherwise.  A probability is at most kMost, inside f16 and as exact as any other
+// relative to its own size, and the sum of a row is at least 1, the weight of the key that m came from.
 //
 // Rows that see different numbers of keys: `limit` is the row's own count, scores at or past it become -inf before the softmax.  Their
 // probability is 0, but 0 x V is NaN for a V that is not finite.  Keys past the last one that any row of the work-group sees are staged as
@@ -24,7 +26,7 @@
 
 namespace pp {
 
-constexpr float kDefer = 8.f;
+constexpr float kMost = 4096.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 #ifdef PP_EMU
@@ -34,28 +36,34 @@ __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 #endif
 
 #ifdef PP_EMU
-inline int opaque_uniform(int v) { return v; }
 inline void keep_branch() {}
 inline void pin(float&) {}
 inline void pin(unsigned&) {}
 #else
-__device__ __forceinline__ int opaque_uniform(int v) {
-  v = __builtin_amdgcn_readfirstlane(v);
-  asm volatile("" : "+s"(v));
-  return v;
-}
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }  // the value is computed by here
 __device__ __forceinline__ void pin(unsigned& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }  // what follows is not computed ahead of its condition
 #endif
-// 16 bytes of global memory (a pointer that may be pp_zero16's would otherwise become a flat access, which counts as an LDS one too)
-__device__ __forceinline__ u4 load_global16(const void* src) {
+// A block of rows that is read 16 bytes at a time; what starts behind its last byte reads as zeros.  The base is wave-uniform, a lane's
+// byte offset the same in every block: no address arithmetic on the vector ALU.
 #ifdef PP_EMU
-  return *static_cast<const u4*>(src);
-#else
-  return *(const __attribute__((address_space(1))) u4*)src;
-#endif
+struct Rows16 {
+  const char* base;
+  unsigned bytes;
+};
+inline Rows16 rows16(const void* base, unsigned bytes) { return Rows16{static_cast<const char*>(base), bytes}; }
+inline u4 load_row16(const Rows16& r, unsigned off) {
+  return (uint64_t)off + 16 <= r.bytes ? *reinterpret_cast<const u4*>(r.base + off) : u4{0u, 0u, 0u, 0u};
 }
+#else
+typedef __amdgpu_buffer_rsrc_t Rows16;
+__device__ __forceinline__ Rows16 rows16(const void* base, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00027000);
+}
+__device__ __forceinline__ u4 load_row16(Rows16 r, unsigned off) {
+  return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+#endif
 
 // 16-bit operand types travel as h8 bit patterns
 template <typename T>
@@ -197,11 +205,11 @@ struct AttnTile {
           for (int rb = 0; rb < RB; ++rb) o[rb][db] = Op<T>::mfma(a, p[rb][sub].f[m], o[rb][db]);
         }
   }
-  // A whole step: w = K Q^T, o += V^T z, y = exp2(x sc + nm) with its sums added to l, mx = row maxima of w.  The MFMAs are laid out one
-  // fragment at a time, each followed by its share of the exponentials (and, once w is complete, of the maxima), and the
-  // LDS reads run kAhead fragments ahead: left to itself the compiler puts all the vector work behind the last MFMA, and waits for each read.
+  // A whole step: w = K Q^T, o += V^T z, y = exp2(x sc + nm) with its sums in bs.  The MFMAs are laid out one fragment at a time, each
+  // followed by its share of the exponentials, and the LDS reads run kAhead fragments ahead: left to itself the compiler puts all the vector
+  // work behind the last MFMA, and waits for each read.
   __device__ __forceinline__ void products(int slot, f16v (&w)[RB][NS], const P (&z)[RB][NS], f16v (*o)[kDB], const f16v (&x)[RB][NS],
-                                           P (&y)[RB][NS], const float* nm, float sc, float* l, float* mx) const {
+                                           P (&y)[RB][NS], const float* nm, float sc, float* bs) const {
     constexpr int n1 = NS * kQF, n2 = NS * 2 * kDB, n = n1 + n2, kAhead = 3, kRing = kAhead + 1;
     constexpr int kEl = RB * NS * 16;
     h8 ring[kRing];
@@ -211,7 +219,17 @@ struct AttnTile {
       return v_frag(slot, i / (2 * kDB), i % kDB, i / kDB % 2);
     };
     u4 yw[RB][NS][2];
-    float even = 0.f, top[RB];
+    float v[kEl];
+    auto take = [&](int e) __attribute__((always_inline)) {  // one exponential behind: its result is not waited for
+      const int rb = e / (16 * NS), sub = e / 16 % NS, r = e % 16;
+      bs[rb] = e % (16 * NS) == 0 ? v[e] : bs[rb] + v[e];
+      pin(bs[rb]);
+      if (r % 2) {
+        unsigned two = Op<T>::pack(v[e - 1], v[e]);
+        pin(two);
+        yw[rb][sub][r / 8][r % 8 / 2] = two;
+      }
+    };
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) ring[j] = fragment(j);
 #pragma unroll
@@ -231,39 +249,18 @@ struct AttnTile {
 #pragma unroll
       for (int e = kEl * j / n; e < kEl * (j + 1) / n; ++e) {
         const int rb = e / (16 * NS), sub = e / 16 % NS, r = e % 16;
-        const float v = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
-        l[rb] += v;
-        pin(l[rb]);
-        if (r % 2) {
-          unsigned two = Op<T>::pack(even, v);
-          pin(two);
-          yw[rb][sub][r / 8][r % 8 / 2] = two;
-        } else {
-          even = v;
-        }
-      }
-      if (j > n1) {
-#pragma unroll
-        for (int e = kEl * (j - n1 - 1) / (n2 - 1); e < kEl * (j - n1) / (n2 - 1); ++e) {
-          const int rb = e / (16 * NS), i = e % (16 * NS);
-          top[rb] = i == 0 ? w[rb][0][0] : fmaxf(top[rb], w[rb][i / 16][i % 16]);
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          if (kEl * (j - n1) / (n2 - 1) > rb * 16 * NS) pin(top[rb]);
+        v[e] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+        if (e > 0) take(e - 1);
       }
       pp_sched_fence();
     }
+    take(kEl - 1);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      mx[rb] = pair32_max(top[rb]);
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          y[rb][sub].f[m] = __builtin_bit_cast(h8, yw[rb][sub][m]);
-        }
-    }
+        for (int m = 0; m < 2; ++m) y[rb][sub].f[m] = __builtin_bit_cast(h8, yw[rb][sub][m]);
   }
   // zeroes what is not finite (exponent all ones: adding one to it carries out of the field); was there any?
   static __device__ __forceinline__ bool scrub(u4& w) {
@@ -348,17 +345,15 @@ struct AttnTile<float, DP, RB_, NS_> {
       for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
   }
   __device__ __forceinline__ void products(int slot, f16v (&w)[1][1], const P (&z)[1][1], f16v (*o)[kDB], const f16v (&x)[1][1],
-                                           P (&y)[1][1], const float* nm, float sc, float* l, float* mx) const {
+                                           P (&y)[1][1], const float* nm, float sc, float* bs) const {
     qk(slot, w);
-    float top = w[0][0][0];
+    bs[0] = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       y[0][0].f[r] = fast_exp2(__builtin_fmaf(x[0][0][r], sc, nm[0]));
-      l[0] += y[0][0].f[r];
-      top = fmaxf(top, w[0][0][r]);
+      bs[0] += y[0][0].f[r];
     }
     pv(slot, z, o);
-    mx[0] = pair32_max(top);
   }
   static __device__ __forceinline__ bool scrub(u4& w) {
     bool any = false;
@@ -412,33 +407,31 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   const int nsteps = (lim.nkeys + BN - 1) / BN;
   if (nsteps <= 0) return;
 
-  // ---- staging: thread -> (row, 16-byte piece) of a block
-  int prow[Tile::kStage], ppiece[Tile::kStage];
-  int64_t koff[Tile::kStage], voff[Tile::kStage];
+  // ---- staging: thread -> 16-byte pieces of a block; a piece past the head dim has an offset that no block reaches
+  unsigned koff[Tile::kStage], voff[Tile::kStage];
 #pragma unroll
   for (int i = 0; i < Tile::kStage; ++i) {
-    const int at = (int)threadIdx.x + 256 * i;
-    prow[i] = at / Tile::kPieces;
-    ppiece[i] = at - prow[i] * Tile::kPieces;
-    koff[i] = prow[i] * k_row + ppiece[i] * Tile::kPer;
-    voff[i] = prow[i] * v_row + ppiece[i] * Tile::kPer;
-    if (ppiece[i] * Tile::kPer >= D) prow[i] = 1 << 30;  // a piece past the head dim is zeros
+    const int at = (int)threadIdx.x + 256 * i, row = at / Tile::kPieces, piece = at - row * Tile::kPieces;
+    const bool in = piece * Tile::kPer < D && row < BN;
+    koff[i] = in ? (unsigned)(row * k_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
+    voff[i] = in ? (unsigned)(row * v_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
   }
   const int mixed_from = lim.group_min;  // from this key on some rows see what others do not
   volatile int* const flag = reinterpret_cast<volatile int*>(reinterpret_cast<unsigned char*>(t.smem) + Tile::kFlag);
   if (threadIdx.x == 0) *flag = 0;
-  const T* const zero = reinterpret_cast<const T*>(pp_zero16);
+  auto block_of = [&](const T* base, int64_t stride, int i) __attribute__((always_inline)) -> Rows16 {
+    const int left = lim.nkeys - i * BN < BN ? lim.nkeys - i * BN : BN;
+    return rows16(base + (int64_t)i * BN * stride, left > 0 ? (unsigned)((left - 1) * stride + D) * (unsigned)sizeof(T) : 0u);
+  };
   auto load_k = [&](u4* dst, int i) __attribute__((always_inline)) {
-    const T* base = k + (int64_t)i * BN * k_row;
-    const int left = lim.nkeys - i * BN;
+    const Rows16 block = block_of(k, k_row, i);
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) dst[j] = load_global16(prow[j] < left ? base + koff[j] : zero);
+    for (int j = 0; j < Tile::kStage; ++j) dst[j] = load_row16(block, koff[j]);
   };
   auto load_v = [&](int i) __attribute__((always_inline)) {
-    const T* base = v + (int64_t)i * BN * v_row;
-    const int left = lim.nkeys - i * BN;
+    const Rows16 block = block_of(v, v_row, i);
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = load_global16(prow[j] < left ? base + voff[j] : zero);
+    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = load_row16(block, voff[j]);
   };
   auto store_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -457,63 +450,45 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
 
   typedef f16v Scores[RB][NS];
   typedef P Probs[RB][NS];
-  // scores of the block whose softmax is next, and their largest per row; probabilities of the block before it.  The second pair takes
-  // turns in the fast steps, so that nothing is copied.
+  // scores of the block whose softmax is next; probabilities of the block before it.  The second pair takes turns in the fast steps, so
+  // that nothing is copied.
   Scores s, s2;
   Probs p, p2;
-  float mx[RB];
-  auto block_max = [&](const Scores& x) __attribute__((always_inline)) {
+  float nm[RB], bs[RB];  // -m sc (NaN before the first visible key: whatever a block holds, it is taken again); sums over the block
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) nm[rb] = __builtin_nanf("");
+  // moves the maximum to that of x and what was summed up with it; x -> y, bs
+  auto move_max = [&](const Scores& x, Probs& y) __attribute__((always_inline)) {
+    keep_branch();
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      float y = x[rb][0][0];
+      float top = x[rb][0][0];
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) y = fmaxf(y, x[rb][sub][r]);
-      mx[rb] = pair32_max(y);
-    }
-  };
-  float alpha[RB], nm[RB];
-  // the maximum moves if a row's passed it by more than kDefer; what was summed up to here is rescaled behind the block's products
-  auto move_max = [&]() __attribute__((always_inline)) -> int {
-    bool moved = false;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) moved |= (mx[rb] - st.m[rb]) * sc > kDefer;  // (-inf) - (-inf) is NaN: moves nothing
-    const int any = wave_any(moved);
-    if (any) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const float mt = fmaxf(st.m[rb], mx[rb]);
-        alpha[rb] = mt == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - mt) * sc);
-        st.l[rb] *= alpha[rb];
-        st.m[rb] = mt;
-        nm[rb] = mt == neg_inf() ? 0.f : -mt * sc;
-      }
-    }
-    return opaque_uniform(any);  // (or the compiler would make two copies of the block's products)
-  };
-  auto rescale = [&]() __attribute__((always_inline)) {
-    keep_branch();
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[rb][sub][r]);
+      top = fmaxf(st.m[rb], pair32_max(top));
+      const float alpha = top == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - top) * sc);
+      const float use = top == neg_inf() ? 0.f : -top * sc;
+      st.m[rb] = top;
+      st.l[rb] *= alpha;
+      nm[rb] = top == neg_inf() ? __builtin_nanf("") : use;
 #pragma unroll
       for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha[rb];
-  };
-  auto softmax = [&](const Scores& x, Probs& to) __attribute__((always_inline)) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+        for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha;
+      bs[rb] = 0.f;
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub) {
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
-          st.l[rb] += e[r];
+          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, use));
+          bs[rb] += e[r];
         }
-        to[rb][sub] = Tile::pack_p(e);
+        y[rb][sub] = Tile::pack_p(e);
       }
+    }
   };
   auto stage = [&](int i, int slot) __attribute__((always_inline)) {
     store_k(slot);  // block i + 2
@@ -527,9 +502,13 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     constexpr int S0 = decltype(slot)::value, S1 = 1 - S0;
     stage(i, S0);
     if (lim.wave_max > 0) {
-      const int moved = move_max();
-      t.products(S1, w, z, st.o, x, y, nm, sc, st.l, mx);
-      if (moved) rescale();
+      t.products(S1, w, z, st.o, x, y, nm, sc, bs);
+      bool over = false;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) over |= !(bs[rb] <= kMost);
+      if (wave_any(over)) move_max(x, y);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) st.l[rb] += bs[rb];
     }
     pp_barrier();
   };
@@ -552,9 +531,9 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
         }
-      block_max(s);
-      if (move_max()) rescale();
-      softmax(s, p);
+      move_max(s, p);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) st.l[rb] += bs[rb];
       if ((i + 1) * BN < lim.wave_max) t.qk(s1, s);
     }
     pp_barrier();
@@ -580,17 +559,13 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   t.qk(0, s);
   pp_barrier();
   const int nfast = mixed_from / BN;
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) alpha[rb] = 1.f, nm[rb] = 0.f;
   for (int i = 0; i < nsteps;) {
     any_step(i);
-    if (++i == 1 && i + 2 <= nfast) {
-      block_max(s);
+    if (++i == 1)
       for (; i + 2 <= nfast; i += 2) {
         fast_step(i, std::integral_constant<int, 1>{}, s, s2, p, p2);
         fast_step(i + 1, std::integral_constant<int, 0>{}, s2, s, p2, p);
       }
-    }
   }
   if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o);
 #pragma unroll
