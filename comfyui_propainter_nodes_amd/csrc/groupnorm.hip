@@ -27,39 +27,68 @@ struct GroupNormK {
   float eps, act_param;
 };
 
+// V consecutive elements: as they are loaded, and as floats
 template <typename T, int V>
-struct Vec;
+struct Vec {  // 16 bytes
+  typedef u4 Raw;
+  static_assert(V * sizeof(T) == 16, "");
+  static __device__ __forceinline__ Raw ld(const T* p) { return *reinterpret_cast<const u4*>(p); }
+  static __device__ __forceinline__ void floats(Raw r, float* f) {
+    if constexpr (V == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(float, (unsigned)r[i]);
+    } else {
+      ld8(reinterpret_cast<const T*>(&r), f);
+    }
+  }
+  static __device__ __forceinline__ void st(T* p, const float* f) {
+    if constexpr (V == 4) *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
+    else st8(p, f);
+  }
+};
 template <typename T>
 struct Vec<T, 1> {
-  static __device__ __forceinline__ void ld(const T* p, float* f) { f[0] = to_f32(*p); }
+  typedef T Raw;
+  static __device__ __forceinline__ Raw ld(const T* p) { return *p; }
+  static __device__ __forceinline__ void floats(Raw r, float* f) { f[0] = to_f32(r); }
   static __device__ __forceinline__ void st(T* p, const float* f) { *p = from_f32<T>(f[0]); }
 };
-template <typename T>
-struct Vec<T, 8> {
-  static __device__ __forceinline__ void ld(const T* p, float* f) { ld8(p, f); }
-  static __device__ __forceinline__ void st(T* p, const float* f) { st8(p, f); }
-};
-template <>
-struct Vec<float, 4> {
-  static __device__ __forceinline__ void ld(const float* p, float* f) {
-    const f4 v = *reinterpret_cast<const f4*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = v[i];
-  }
-  static __device__ __forceinline__ void st(float* p, const float* f) { *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]}; }
-};
 
+// x Phi(x) = max(x, 0) - z Q(z), z = |x|, Q(z) = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) R(t), t = 1 / (1 + 0.3 z): R is a polynomial fitted to
+// erfcx(z / sqrt 2) / 2 over z in [0, 14], 1.5e-7 off at most relative to Q (so both tails keep their relative accuracy).  16 operations; the
+// library's erff made the 16-bit apply pass three times as long as its memory traffic.
+__device__ __forceinline__ float gelu_fast(float x) {
+  const float z = fminf(fabsf(x), 20.f);
+  const float t = fast_rcp(__builtin_fmaf(z, 0.3f, 1.f));
+  float r = 0.03567391261458397f;
+  r = __builtin_fmaf(r, t, -0.157199427485466f);
+  r = __builtin_fmaf(r, t, 0.2063470482826233f);
+  r = __builtin_fmaf(r, t, -0.05367753654718399f);
+  r = __builtin_fmaf(r, t, 0.12855829298496246f);
+  r = __builtin_fmaf(r, t, 0.0999145358800888f);
+  r = __builtin_fmaf(r, t, 0.12075378000736237f);
+  r = __builtin_fmaf(r, t, 0.11962930858135223f);
+  const float q = __expf(-0.5f * z * z) * (r * t);
+  const float y = __builtin_fmaf(-z, q, x > 0.f ? x : 0.f);
+  return x != x ? x : y;
+}
+
+// f32 storage: the library's functions; 16-bit storage: hardware exponential and reciprocal (a few 2^-24, far below the rounding to come)
+template <typename T>
 __device__ __forceinline__ float norm_act(float v, int act, float param) {
+  constexpr bool kExact = sizeof(T) == 4;
   switch (act) {
     case PP_ACT_RELU: return v > 0.f || v != v ? v : 0.f;
     case PP_ACT_LEAKY: return v > 0.f ? v : v * param;
-    case PP_ACT_SIGMOID: return 1.f / (1.f + expf(-v));
+    case PP_ACT_SIGMOID: return kExact ? 1.f / (1.f + expf(-v)) : sigmoidf_(v);
     case PP_ACT_TANH: return tanhf(v);
-    case PP_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-    case PP_ACT_SILU: return v / (1.f + expf(-v));
+    case PP_ACT_GELU: return kExact ? 0.5f * v * (1.f + erff(v * 0.70710678118654752f)) : gelu_fast(v);
+    case PP_ACT_SILU: return kExact ? v / (1.f + expf(-v)) : v * sigmoidf_(v);
     default: return v;
   }
 }
+
+constexpr int kAhead = 4;  // 16-byte loads of a thread in flight
 
 // sums of one chunk of one image, all groups
 template <typename T, int V>
@@ -76,17 +105,30 @@ __global__ void __launch_bounds__(256) groupnorm_sums_kernel(const GroupNormK k)
     double s[V], q[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = q[e] = 0.0;
+    auto add = [&](typename Vec<T, V>::Raw raw) __attribute__((always_inline)) {
+      float v[V];
+      Vec<T, V>::floats(raw, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double d = (double)v[e];
+        s[e] += d;
+        q[e] += d * d;
+      }
+    };
     if (pl < k.lanes && col < allcols) {
       const T* base = (const T*)k.x + (int64_t)n * k.HW * k.x_ldc + (int64_t)col * V;
-      for (int64_t p = p0 + pl; p < p1; p += k.lanes) {
-        float v[V];
-        Vec<T, V>::ld(base + p * k.x_ldc, v);
+      const int64_t step = (int64_t)k.lanes * k.x_ldc;
+      int64_t p = p0 + pl;
+      const T* at = base + p * k.x_ldc;
+      for (; p + (kAhead - 1) * k.lanes < p1; p += kAhead * k.lanes, at += kAhead * step) {
+        typename Vec<T, V>::Raw v[kAhead];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const double d = (double)v[e];
-          s[e] += d;
-          q[e] += d * d;
-        }
+        for (int u = 0; u < kAhead; ++u) v[u] = Vec<T, V>::ld(at + u * step);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) add(v[u]);
+      }
+      for (; p < p1; p += k.lanes, at += step) {
+        add(Vec<T, V>::ld(at));
       }
     }
     __syncthreads();  // the previous pass's readers
@@ -96,17 +138,23 @@ __global__ void __launch_bounds__(256) groupnorm_sums_kernel(const GroupNormK k)
       sh[(tid * V + e) * 2 + 1] = q[e];
     }
     __syncthreads();
-    // groups that touch channels [a, b): thread g % 256 owns group g in every pass, so the running sums need no exchange
-    const int a = c0 * V, b = (c0 + k.cols) * V < k.C ? (c0 + k.cols) * V : k.C;
+    // a channel's pixel lanes, then a group's channels: thread g % 256 owns group g in every pass, so the running sums need no exchange
+    const int wide = k.cols * V;
+    for (int c = tid; c < wide; c += 256)
+      for (int l = 1; l < k.lanes; ++l) {
+        sh[2 * c] += sh[(l * wide + c) * 2];
+        sh[2 * c + 1] += sh[(l * wide + c) * 2 + 1];
+      }
+    __syncthreads();
+    const int a = c0 * V, b = a + wide < k.C ? a + wide : k.C;
     for (int g = tid; g < k.G; g += 256) {
       const int lo = a > g * k.cpg ? a : g * k.cpg, hi = b < (g + 1) * k.cpg ? b : (g + 1) * k.cpg;
       if (lo >= hi) continue;
       double ss = 0.0, qq = 0.0;
-      for (int l = 0; l < k.lanes; ++l)
-        for (int c = lo; c < hi; ++c) {
-          ss += sh[(l * k.cols * V + c - a) * 2];
-          qq += sh[(l * k.cols * V + c - a) * 2 + 1];
-        }
+      for (int c = lo; c < hi; ++c) {
+        ss += sh[(c - a) * 2];
+        qq += sh[(c - a) * 2 + 1];
+      }
       if (lo != g * k.cpg) {
         ss += dst[2 * g];
         qq += dst[2 * g + 1];
@@ -125,22 +173,63 @@ __device__ __forceinline__ f4 finish_stats(double s, double q, double m, float e
   return f4{hi, (float)(mean - (double)hi), (float)(1.0 / sqrt(var + (double)eps)), 0.f};
 }
 
+// sum over the lanes of a wave, the same order for every lane
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = __builtin_bit_cast(unsigned, shfl_xor(__builtin_bit_cast(float, (unsigned)u), m));
+    const unsigned hi = __builtin_bit_cast(unsigned, shfl_xor(__builtin_bit_cast(float, (unsigned)(u >> 32)), m));
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  }
+  return v;
+}
+
+// a wave per (image, group): its lanes share the chunks
 __global__ void __launch_bounds__(256) groupnorm_finish_kernel(const GroupNormK k) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= (int64_t)k.N * k.G) return;
   const int64_t n = i / k.G, g = i - n * k.G;
   const double* src = k.partials + (n * k.nchunks * k.G + g) * 2;
   double s = 0.0, q = 0.0;
-  for (int c = 0; c < k.nchunks; ++c) {
+  for (int c = lane_id(); c < k.nchunks; c += 64) {
     s += src[(int64_t)c * k.G * 2];
     q += src[(int64_t)c * k.G * 2 + 1];
   }
-  reinterpret_cast<f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2)[i] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
+  s = wave_sum(s);
+  q = wave_sum(q);
+  if (lane_id() == 0)
+    reinterpret_cast<f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2)[i] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
 }
 
+template <int V>
+struct Affine {  // what a vector of V channels needs
+  float mh[V], ml[V], a[V], b[V];
+  __device__ __forceinline__ void set(const GroupNormK& k, int c, int e, f4 st) {
+    mh[e] = st[0];
+    ml[e] = st[1];
+    a[e] = k.gamma ? st[2] * k.gamma[c] : st[2];
+    b[e] = k.beta ? k.beta[c] : 0.f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void apply(const GroupNormK& k, typename Vec<T, V>::Raw x, typename Vec<T, V>::Raw skip, T* dst) const {
+    float v[V], sk[V];
+    Vec<T, V>::floats(x, v);
+    if (k.skip) Vec<T, V>::floats(skip, sk);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[e] = norm_act<T>(((v[e] - mh[e]) - ml[e]) * a[e] + b[e], k.act, k.act_param);
+      if (k.skip) v[e] += sk[e];
+      if (k.relu_post) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;
+    }
+    Vec<T, V>::st(dst, v);
+  }
+};
+
+// Chunks are taken in the opposite order of the sums: what they read last is still in the cache.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k) {
-  const int n = (int)blockIdx.x / k.nchunks, chunk = (int)blockIdx.x - n * k.nchunks;
+  const int id = (int)(gridDim.x - 1 - blockIdx.x), n = id / k.nchunks, chunk = id - n * k.nchunks;
   const int tid = (int)threadIdx.x;
   const int64_t p0 = (int64_t)chunk * k.per, p1 = p0 + k.per < k.HW ? p0 + k.per : k.HW;
   const f4* stats = reinterpret_cast<const f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2) + (int64_t)n * k.G;
@@ -148,30 +237,79 @@ __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k
   const int allcols = (k.C + V - 1) / V;
   if (pl >= k.lanes) return;
   for (int col = cv; col < allcols; col += k.cols) {
-    float mh[V], ml[V], a[V], b[V];
+    Affine<V> f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = col * V + e;
-      const f4 st = stats[c / k.cpg];
-      mh[e] = st[0];
-      ml[e] = st[1];
-      a[e] = k.gamma ? st[2] * k.gamma[c] : st[2];
-      b[e] = k.beta ? k.beta[c] : 0.f;
-    }
+    for (int e = 0; e < V; ++e) f.set(k, col * V + e, e, stats[(col * V + e) / k.cpg]);
     const int64_t px = (int64_t)n * k.HW, c0 = (int64_t)col * V;
-    for (int64_t p = p0 + pl; p < p1; p += k.lanes) {
-      float v[V], sk[V];
-      Vec<T, V>::ld((const T*)k.x + (px + p) * k.x_ldc + c0, v);
-      if (k.skip) Vec<T, V>::ld((const T*)k.skip + (px + p) * k.skip_ldc + c0, sk);
+    const T* x = (const T*)k.x + px * k.x_ldc + c0;
+    const T* skip = (const T*)k.skip + px * k.skip_ldc + c0;
+    T* y = (T*)k.y + px * k.y_ldc + c0;
+    int64_t p = p0 + pl;
+    for (; p + (kAhead - 1) * k.lanes < p1; p += kAhead * k.lanes) {
+      typename Vec<T, V>::Raw v[kAhead], sk[kAhead];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[e] = norm_act(((v[e] - mh[e]) - ml[e]) * a[e] + b[e], k.act, k.act_param);
-        if (k.skip) v[e] += sk[e];
-        if (k.relu_post) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;
+      for (int u = 0; u < kAhead; ++u) {
+        v[u] = Vec<T, V>::ld(x + (p + u * k.lanes) * k.x_ldc);
+        sk[u] = v[u];
+        if (k.skip) sk[u] = Vec<T, V>::ld(skip + (p + u * k.lanes) * k.skip_ldc);
       }
-      Vec<T, V>::st((T*)k.y + (px + p) * k.y_ldc + c0, v);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) f.apply(k, v[u], sk[u], y + (p + u * k.lanes) * k.y_ldc);
+    }
+    for (; p < p1; p += k.lanes) {
+      const auto v = Vec<T, V>::ld(x + p * k.x_ldc);
+      f.apply(k, v, k.skip ? Vec<T, V>::ld(skip + p * k.skip_ldc) : v, y + p * k.y_ldc);
     }
   }
+}
+
+// One launch: a work-group keeps all of a group (at most 256 kHeld vectors, each inside the group) in registers between the statistics
+// and the values, so x is read once.
+constexpr int kHeld = 8;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) groupnorm_held_kernel(const GroupNormK k) {
+  __shared__ double sh[8];
+  const int n = (int)blockIdx.x / k.G, g = (int)blockIdx.x - n * k.G;
+  const int tid = (int)threadIdx.x, per = k.cpg / V, total = (int)k.HW * per;
+  const int64_t px = (int64_t)n * k.HW, c0 = (int64_t)g * k.cpg;
+  typename Vec<T, V>::Raw v[kHeld];
+  int at[kHeld];
+  double s = 0.0, q = 0.0;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    at[u] = tid + 256 * u;
+    if (at[u] < total) v[u] = Vec<T, V>::ld((const T*)k.x + (px + at[u] / per) * k.x_ldc + c0 + at[u] % per * V);
+  }
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (at[u] < total) {
+      float f[V];
+      Vec<T, V>::floats(v[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double d = (double)f[e];
+        s += d;
+        q += d * d;
+      }
+    }
+  s = wave_sum(s);
+  q = wave_sum(q);
+  if ((tid & 63) == 0) {
+    sh[tid >> 6] = s;
+    sh[4 + (tid >> 6)] = q;
+  }
+  __syncthreads();
+  const f4 st = finish_stats(sh[0] + sh[1] + sh[2] + sh[3], sh[4] + sh[5] + sh[6] + sh[7], (double)k.HW * k.cpg, k.eps);
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (at[u] < total) {
+      const int64_t p = px + at[u] / per, c = c0 + at[u] % per * V;
+      Affine<V> f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) f.set(k, (int)c + e, e, st);
+      f.apply(k, v[u], k.skip ? Vec<T, V>::ld((const T*)k.skip + p * k.skip_ldc + c) : v[u], (T*)k.y + p * k.y_ldc + c);
+    }
 }
 
 }  // namespace pp
@@ -179,6 +317,10 @@ __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k
 template <typename T, int V>
 static int launch_groupnorm(void* stream, pp::GroupNormK& k) {
   using namespace pp;
+  if (k.cpg % V == 0 && k.HW * (k.cpg / V) <= 256 * kHeld && k.N * k.G < (1 << 23)) {
+    PP_LAUNCH((groupnorm_held_kernel<T, V>), dim3((unsigned)(k.N * k.G)), dim3(256), 0, stream, k);
+    return pp_check_launch("pp_groupnorm(held)");
+  }
   const int allcols = (k.C + V - 1) / V;
   k.cols = allcols < 256 ? allcols : 256;
   k.lanes = 256 / k.cols;
@@ -186,7 +328,7 @@ static int launch_groupnorm(void* stream, pp::GroupNormK& k) {
   PP_LAUNCH((groupnorm_sums_kernel<T, V>), grid, dim3(256), 0, stream, k);
   int rc = pp_check_launch("pp_groupnorm(sums)");
   if (rc != PP_OK) return rc;
-  PP_LAUNCH(groupnorm_finish_kernel, dim3(pp_blocks_1d((int64_t)k.N * k.G)), dim3(256), 0, stream, k);
+  PP_LAUNCH(groupnorm_finish_kernel, dim3((unsigned)(((int64_t)k.N * k.G + 3) / 4)), dim3(256), 0, stream, k);
   rc = pp_check_launch("pp_groupnorm(finish)");
   if (rc != PP_OK) return rc;
   PP_LAUNCH((groupnorm_apply_kernel<T, V>), grid, dim3(256), 0, stream, k);
