@@ -23,9 +23,15 @@ struct GroupNormK {
   int64_t x_ldc, y_ldc, skip_ldc, HW;
   int64_t per;  // pixels of a chunk
   int N, C, G, cpg, nchunks, cols, lanes;  // cols: column vectors of a work-group pass, lanes: pixels that it takes at once
-  int act, relu_post;
+  int relu_post, join;
   float eps, act_param;
 };
+
+#ifdef PP_EMU
+inline float fast_exp2_(float x) { return exp2f(x); }
+#else
+__device__ __forceinline__ float fast_exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+#endif
 
 // V consecutive elements: as they are loaded, and as floats
 template <typename T, int V>
@@ -54,28 +60,27 @@ struct Vec<T, 1> {
   static __device__ __forceinline__ void st(T* p, const float* f) { *p = from_f32<T>(f[0]); }
 };
 
-// x Phi(x) = max(x, 0) - z Q(z), z = |x|, Q(z) = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) R(t), t = 1 / (1 + 0.3 z): R is a polynomial fitted to
-// erfcx(z / sqrt 2) / 2 over z in [0, 14], 1.5e-7 off at most relative to Q (so both tails keep their relative accuracy).  16 operations; the
-// library's erff made the 16-bit apply pass three times as long as its memory traffic.
+// x Phi(x) = max(x, 0) - z Q(z), z = |x|, Q(z) = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) R(t), t = 1 / (1 + 0.36 z): R is a polynomial fitted to
+// erfcx(z / sqrt 2) / 2 over z in [0, 14], 9e-7 off at most relative to Q (so both tails keep their relative accuracy).  max(x, 0) is
+// (x + |x|) / 2, which a NaN passes.
 __device__ __forceinline__ float gelu_fast(float x) {
   const float z = fminf(fabsf(x), 20.f);
-  const float t = fast_rcp(__builtin_fmaf(z, 0.3f, 1.f));
-  float r = 0.03567391261458397f;
-  r = __builtin_fmaf(r, t, -0.157199427485466f);
-  r = __builtin_fmaf(r, t, 0.2063470482826233f);
-  r = __builtin_fmaf(r, t, -0.05367753654718399f);
-  r = __builtin_fmaf(r, t, 0.12855829298496246f);
-  r = __builtin_fmaf(r, t, 0.0999145358800888f);
-  r = __builtin_fmaf(r, t, 0.12075378000736237f);
-  r = __builtin_fmaf(r, t, 0.11962930858135223f);
-  const float q = __expf(-0.5f * z * z) * (r * t);
-  const float y = __builtin_fmaf(-z, q, x > 0.f ? x : 0.f);
-  return x != x ? x : y;
+  const float t = fast_rcp(__builtin_fmaf(z, 0.36f, 1.f));
+  float r = 0.04705524072051048f;
+  r = __builtin_fmaf(r, t, -0.17976124584674835f);
+  r = __builtin_fmaf(r, t, 0.18094944953918457f);
+  r = __builtin_fmaf(r, t, 0.02655242383480072f);
+  r = __builtin_fmaf(r, t, 0.13971813023090363f);
+  r = __builtin_fmaf(r, t, 0.14177265763282776f);
+  r = __builtin_fmaf(r, t, 0.14371302723884583f);
+  const float u = z * 0.84932180028801907f;  // exp(-z^2 / 2) = 2^(-u^2)
+  const float q = fast_exp2_(-u * u) * (r * t);
+  return __builtin_fmaf(-z, q, __builtin_fmaf(0.5f, fabsf(x), 0.5f * x));
 }
 
 // f32 storage: the library's functions; 16-bit storage: hardware exponential and reciprocal (a few 2^-24, far below the rounding to come)
 template <typename T>
-__device__ __forceinline__ float norm_act(float v, int act, float param) {
+__device__ __forceinline__ float norm_act(float v, int act, float param) {  // act: a compile-time constant or uniform
   constexpr bool kExact = sizeof(T) == 4;
   switch (act) {
     case PP_ACT_RELU: return v > 0.f || v != v ? v : 0.f;
@@ -88,6 +93,8 @@ __device__ __forceinline__ float norm_act(float v, int act, float param) {
   }
 }
 
+constexpr int kOwnGroups = 32;  // groups and sums up to which the apply pass joins them itself
+constexpr int kOwnSums = 2048;
 constexpr int kAhead = 4;  // 16-byte loads of a thread in flight
 
 // sums of one chunk of one image, all groups
@@ -112,7 +119,7 @@ __global__ void __launch_bounds__(256) groupnorm_sums_kernel(const GroupNormK k)
       for (int e = 0; e < V; ++e) {
         const double d = (double)v[e];
         s[e] += d;
-        q[e] += d * d;
+        q[e] = __builtin_fma(d, d, q[e]);
       }
     };
     if (pl < k.lanes && col < allcols) {
@@ -140,11 +147,16 @@ __global__ void __launch_bounds__(256) groupnorm_sums_kernel(const GroupNormK k)
     __syncthreads();
     // a channel's pixel lanes, then a group's channels: thread g % 256 owns group g in every pass, so the running sums need no exchange
     const int wide = k.cols * V;
-    for (int c = tid; c < wide; c += 256)
-      for (int l = 1; l < k.lanes; ++l) {
-        sh[2 * c] += sh[(l * wide + c) * 2];
-        sh[2 * c + 1] += sh[(l * wide + c) * 2 + 1];
+    for (int c = tid; c < wide; c += 256) {
+      double ss = 0.0, qq = 0.0;
+#pragma unroll 4
+      for (int l = 0; l < k.lanes; ++l) {
+        ss += sh[(l * wide + c) * 2];
+        qq += sh[(l * wide + c) * 2 + 1];
       }
+      sh[2 * c] = ss;
+      sh[2 * c + 1] = qq;
+    }
     __syncthreads();
     const int a = c0 * V, b = a + wide < k.C ? a + wide : k.C;
     for (int g = tid; g < k.G; g += 256) {
@@ -202,23 +214,29 @@ __global__ void __launch_bounds__(256) groupnorm_finish_kernel(const GroupNormK 
     reinterpret_cast<f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2)[i] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
 }
 
-template <int V>
-struct Affine {  // what a vector of V channels needs
-  float mh[V], ml[V], a[V], b[V];
+// What a vector of V channels needs: ((x - mh) - ml) a + b; with 16-bit storage x - mh is exact to 2^-24 of the larger one and -ml a goes
+// into b, one operation less per value.
+template <typename T, int V>
+struct Affine {
+  static constexpr bool kLow = sizeof(T) == 4;
+  float mh[V], ml[kLow ? V : 1], a[V], b[V];
   __device__ __forceinline__ void set(const GroupNormK& k, int c, int e, f4 st) {
     mh[e] = st[0];
-    ml[e] = st[1];
     a[e] = k.gamma ? st[2] * k.gamma[c] : st[2];
     b[e] = k.beta ? k.beta[c] : 0.f;
+    if constexpr (kLow) ml[e] = st[1];
+    else b[e] = __builtin_fmaf(-st[1], a[e], b[e]);
   }
-  template <typename T>
+  template <int ACT>
   __device__ __forceinline__ void apply(const GroupNormK& k, typename Vec<T, V>::Raw x, typename Vec<T, V>::Raw skip, T* dst) const {
     float v[V], sk[V];
     Vec<T, V>::floats(x, v);
     if (k.skip) Vec<T, V>::floats(skip, sk);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      v[e] = norm_act<T>(((v[e] - mh[e]) - ml[e]) * a[e] + b[e], k.act, k.act_param);
+      float d = v[e] - mh[e];
+      if constexpr (kLow) d -= ml[e];
+      v[e] = norm_act<T>(__builtin_fmaf(d, a[e], b[e]), ACT, k.act_param);
       if (k.skip) v[e] += sk[e];
       if (k.relu_post) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;
     }
@@ -227,17 +245,43 @@ struct Affine {  // what a vector of V channels needs
 };
 
 // Chunks are taken in the opposite order of the sums: what they read last is still in the cache.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k) {
   const int id = (int)(gridDim.x - 1 - blockIdx.x), n = id / k.nchunks, chunk = id - n * k.nchunks;
   const int tid = (int)threadIdx.x;
   const int64_t p0 = (int64_t)chunk * k.per, p1 = p0 + k.per < k.HW ? p0 + k.per : k.HW;
+  __shared__ f4 own[kOwnGroups];
+  __shared__ double sh[512];
   const f4* stats = reinterpret_cast<const f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2) + (int64_t)n * k.G;
+  if (k.join) {  // few enough sums: every work-group joins them itself, a launch less
+    const int G2 = k.G <= 8 ? 8 : k.G <= 16 ? 16 : 32, g = tid % G2, part = tid / G2, parts = 256 / G2;
+    const double* src = k.partials + ((int64_t)n * k.nchunks * k.G + g) * 2;
+    double s = 0.0, q = 0.0;
+    if (g < k.G) {
+#pragma unroll 4
+      for (int c = part; c < k.nchunks; c += parts) {
+        s += src[(int64_t)c * k.G * 2];
+        q += src[(int64_t)c * k.G * 2 + 1];
+      }
+    }
+    sh[2 * tid] = s;
+    sh[2 * tid + 1] = q;
+    __syncthreads();
+    if (tid < k.G) {
+      for (int i = 1; i < parts; ++i) {
+        s += sh[2 * (tid + i * G2)];
+        q += sh[2 * (tid + i * G2) + 1];
+      }
+      own[tid] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
+    }
+    __syncthreads();
+    stats = own;
+  }
   const int pl = tid / k.cols, cv = tid - pl * k.cols;
   const int allcols = (k.C + V - 1) / V;
   if (pl >= k.lanes) return;
   for (int col = cv; col < allcols; col += k.cols) {
-    Affine<V> f;
+    Affine<T, V> f;
 #pragma unroll
     for (int e = 0; e < V; ++e) f.set(k, col * V + e, e, stats[(col * V + e) / k.cpg]);
     const int64_t px = (int64_t)n * k.HW, c0 = (int64_t)col * V;
@@ -254,11 +298,11 @@ __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k
         if (k.skip) sk[u] = Vec<T, V>::ld(skip + (p + u * k.lanes) * k.skip_ldc);
       }
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) f.apply(k, v[u], sk[u], y + (p + u * k.lanes) * k.y_ldc);
+      for (int u = 0; u < kAhead; ++u) f.template apply<ACT>(k, v[u], sk[u], y + (p + u * k.lanes) * k.y_ldc);
     }
     for (; p < p1; p += k.lanes) {
       const auto v = Vec<T, V>::ld(x + p * k.x_ldc);
-      f.apply(k, v, k.skip ? Vec<T, V>::ld(skip + p * k.skip_ldc) : v, y + p * k.y_ldc);
+      f.template apply<ACT>(k, v, k.skip ? Vec<T, V>::ld(skip + p * k.skip_ldc) : v, y + p * k.y_ldc);
     }
   }
 }
@@ -267,7 +311,7 @@ __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k
 // and the values, so x is read once.
 constexpr int kHeld = 8;
 
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) groupnorm_held_kernel(const GroupNormK k) {
   __shared__ double sh[8];
   const int n = (int)blockIdx.x / k.G, g = (int)blockIdx.x - n * k.G;
@@ -290,7 +334,7 @@ __global__ void __launch_bounds__(256) groupnorm_held_kernel(const GroupNormK k)
       for (int e = 0; e < V; ++e) {
         const double d = (double)f[e];
         s += d;
-        q += d * d;
+        q = __builtin_fma(d, d, q);
       }
     }
   s = wave_sum(s);
@@ -305,34 +349,50 @@ __global__ void __launch_bounds__(256) groupnorm_held_kernel(const GroupNormK k)
   for (int u = 0; u < kHeld; ++u)
     if (at[u] < total) {
       const int64_t p = px + at[u] / per, c = c0 + at[u] % per * V;
-      Affine<V> f;
+      Affine<T, V> f;
 #pragma unroll
       for (int e = 0; e < V; ++e) f.set(k, (int)c + e, e, st);
-      f.apply(k, v[u], k.skip ? Vec<T, V>::ld((const T*)k.skip + p * k.skip_ldc + c) : v[u], (T*)k.y + p * k.y_ldc + c);
+      f.template apply<ACT>(k, v[u], k.skip ? Vec<T, V>::ld((const T*)k.skip + p * k.skip_ldc + c) : v[u], (T*)k.y + p * k.y_ldc + c);
     }
 }
 
 }  // namespace pp
 
-template <typename T, int V>
-static int launch_groupnorm(void* stream, pp::GroupNormK& k) {
+template <typename T, int V, int ACT>
+static int launch_groupnorm_act(void* stream, pp::GroupNormK& k) {
   using namespace pp;
-  if (k.cpg % V == 0 && k.HW * (k.cpg / V) <= 256 * kHeld && k.N * k.G < (1 << 23)) {
-    PP_LAUNCH((groupnorm_held_kernel<T, V>), dim3((unsigned)(k.N * k.G)), dim3(256), 0, stream, k);
+  if (k.cpg % V == 0 && k.HW * (k.cpg / V) <= 256 * kHeld && (int64_t)k.N * k.G < (1 << 23)) {
+    PP_LAUNCH((groupnorm_held_kernel<T, V, ACT>), dim3((unsigned)(k.N * k.G)), dim3(256), 0, stream, k);
     return pp_check_launch("pp_groupnorm(held)");
   }
   const int allcols = (k.C + V - 1) / V;
   k.cols = allcols < 256 ? allcols : 256;
   k.lanes = 256 / k.cols;
+  k.join = k.G <= kOwnGroups && (int64_t)k.nchunks * k.G <= kOwnSums;
   const dim3 grid((unsigned)(k.N * k.nchunks));
   PP_LAUNCH((groupnorm_sums_kernel<T, V>), grid, dim3(256), 0, stream, k);
   int rc = pp_check_launch("pp_groupnorm(sums)");
   if (rc != PP_OK) return rc;
-  PP_LAUNCH(groupnorm_finish_kernel, dim3((unsigned)(((int64_t)k.N * k.G + 3) / 4)), dim3(256), 0, stream, k);
-  rc = pp_check_launch("pp_groupnorm(finish)");
-  if (rc != PP_OK) return rc;
-  PP_LAUNCH((groupnorm_apply_kernel<T, V>), grid, dim3(256), 0, stream, k);
+  if (!k.join) {
+    PP_LAUNCH(groupnorm_finish_kernel, dim3((unsigned)(((int64_t)k.N * k.G + 3) / 4)), dim3(256), 0, stream, k);
+    rc = pp_check_launch("pp_groupnorm(finish)");
+    if (rc != PP_OK) return rc;
+  }
+  PP_LAUNCH((groupnorm_apply_kernel<T, V, ACT>), grid, dim3(256), 0, stream, k);
   return pp_check_launch("pp_groupnorm(apply)");
+}
+
+template <typename T, int V>
+static int launch_groupnorm(void* stream, pp::GroupNormK& k, int act) {
+  switch (act) {
+    case PP_ACT_RELU: return launch_groupnorm_act<T, V, PP_ACT_RELU>(stream, k);
+    case PP_ACT_LEAKY: return launch_groupnorm_act<T, V, PP_ACT_LEAKY>(stream, k);
+    case PP_ACT_SIGMOID: return launch_groupnorm_act<T, V, PP_ACT_SIGMOID>(stream, k);
+    case PP_ACT_TANH: return launch_groupnorm_act<T, V, PP_ACT_TANH>(stream, k);
+    case PP_ACT_GELU: return launch_groupnorm_act<T, V, PP_ACT_GELU>(stream, k);
+    case PP_ACT_SILU: return launch_groupnorm_act<T, V, PP_ACT_SILU>(stream, k);
+    default: return launch_groupnorm_act<T, V, PP_ACT_NONE>(stream, k);
+  }
 }
 
 extern "C" int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p) {
@@ -356,12 +416,12 @@ extern "C" int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p) {
   k.x_ldc = p->x_ldc; k.y_ldc = p->y_ldc; k.skip_ldc = p->skip_ldc; k.HW = p->HW;
   k.per = (p->HW + p->nchunks - 1) / p->nchunks;
   k.N = (int)p->N; k.C = (int)p->C; k.G = (int)p->groups; k.cpg = (int)(p->C / p->groups); k.nchunks = (int)p->nchunks;
-  k.act = p->act; k.relu_post = p->relu_post; k.eps = p->eps; k.act_param = p->act_param;
+  k.relu_post = p->relu_post; k.eps = p->eps; k.act_param = p->act_param;
   // 16-byte accesses where every row of every tensor allows them, single elements otherwise
   const int V = p->dtype == PP_F32 ? 4 : 8;
   const bool wide = p->C % V == 0 && p->x_ldc % V == 0 && p->y_ldc % V == 0 && (!p->skip || p->skip_ldc % V == 0) &&
                     (((uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->skip) % 16) == 0;
-  if (p->dtype == PP_F32) return wide ? launch_groupnorm<float, 4>(stream, k) : launch_groupnorm<float, 1>(stream, k);
-  if (p->dtype == PP_F16) return wide ? launch_groupnorm<half_t, 8>(stream, k) : launch_groupnorm<half_t, 1>(stream, k);
-  return wide ? launch_groupnorm<bf16_t, 8>(stream, k) : launch_groupnorm<bf16_t, 1>(stream, k);
+  if (p->dtype == PP_F32) return wide ? launch_groupnorm<float, 4>(stream, k, p->act) : launch_groupnorm<float, 1>(stream, k, p->act);
+  if (p->dtype == PP_F16) return wide ? launch_groupnorm<half_t, 8>(stream, k, p->act) : launch_groupnorm<half_t, 1>(stream, k, p->act);
+  return wide ? launch_groupnorm<bf16_t, 8>(stream, k, p->act) : launch_groupnorm<bf16_t, 1>(stream, k, p->act);
 }

@@ -118,32 +118,65 @@ __global__ void __launch_bounds__(256, Tile::kWaves) prefix_attention_kernel(con
   }
 }
 
-// joins the parts of a row: one thread per 4 head-dim values
-template <typename Tile>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixK a) {
+// Joins the parts of a row: a row's D values are DL threads of 4, and PG groups of such threads take every PG-th part each, four parts'
+// loads in flight; then the groups' results are joined in LDS.  (One thread per 4 values walking all parts took 17 us for 33 parts of 1024 rows.)
+template <typename Tile, int DL>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixK a, int pg_log2) {
   typedef typename Tile::type T;
-  const int per = a.D / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.L * a.H;
-  if (i >= rows * per) return;
-  const int64_t row = i / per;
-  const int d = (int)(i - row * per) * 4;
-  const float* ml = a.part_ml + row * a.parts * 2;
-  const float* po = a.part_o + row * a.parts * a.D + d;
-  float m = neg_inf();
-  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, ml[2 * p]);
-  float l = 0.f;
+  __shared__ f4 so[256];
+  __shared__ float sm[256], sl[256];
+  const int tid = (int)threadIdx.x, dl = tid % DL, PG = 1 << pg_log2, pg = tid / DL % PG, slot = tid / (DL * PG);
+  const int64_t row = (int64_t)blockIdx.x * (256 / (DL * PG)) + slot, rows = (int64_t)a.B * a.L * a.H;
+  const bool live = row < rows && 4 * dl < a.D;
+  float m = neg_inf(), l = 0.f;
   f4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < a.parts; ++p) {
-    const float mp = ml[2 * p];
-    const float w = mp == m ? 1.f : fast_exp2((mp - m) * a.sc);
-    l += w * ml[2 * p + 1];
-    o += w * *reinterpret_cast<const f4*>(po + (int64_t)p * a.D);
+  if (live) {
+    const float* ml = a.part_ml + row * a.parts * 2;
+    const float* po = a.part_o + row * a.parts * a.D + 4 * dl;
+    for (int p0 = pg; p0 < a.parts; p0 += 4 * PG) {
+      float pm[4], pl[4];
+      f4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int p = p0 + u * PG;
+        const bool in = p < a.parts;
+        pm[u] = in ? ml[2 * p] : neg_inf();
+        pl[u] = in ? ml[2 * p + 1] : 0.f;
+        v[u] = in ? *reinterpret_cast<const f4*>(po + (int64_t)p * a.D) : f4{0.f, 0.f, 0.f, 0.f};
+      }
+      const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+      const float w = m == top ? 1.f : fast_exp2((m - top) * a.sc);
+      m = top;
+      l *= w;
+      o *= w;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float x = pm[u] == top ? 1.f : fast_exp2((pm[u] - top) * a.sc);
+        l += x * pl[u];
+        o += x * v[u];
+      }
+    }
+  }
+  so[tid] = o;
+  sm[tid] = m;
+  sl[tid] = l;
+  __syncthreads();
+  if (!live || pg != 0) return;
+  float top = m;
+  for (int g = 1; g < PG; ++g) top = fmaxf(top, sm[tid + g * DL]);
+  const float w = m == top ? 1.f : fast_exp2((m - top) * a.sc);
+  l *= w;
+  o *= w;
+  for (int g = 1; g < PG; ++g) {
+    const float x = sm[tid + g * DL] == top ? 1.f : fast_exp2((sm[tid + g * DL] - top) * a.sc);
+    l += x * sl[tid + g * DL];
+    o += x * so[tid + g * DL];
   }
   const int64_t bl = row / a.H, head = row - bl * a.H, b = bl / a.L, tok = bl - b * a.L;
   // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
   const int64_t own = a.own_len[b] > a.S ? a.S : a.own_len[b];
   const float inv = a.P > 0 || own - a.L + tok + 1 > 0 ? 1.f / l : 0.f;
-  Tile::store4((T*)a.out + b * a.out_seq + tok * a.out_row + head * a.out_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  Tile::store4((T*)a.out + b * a.out_seq + tok * a.out_row + head * a.out_head + 4 * dl, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 }  // namespace pp
@@ -161,7 +194,12 @@ static int launch_prefix(void* stream, pp::PrefixK& a) {
   if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(256), Tile::kSmem, stream, a);
   const int rc = pp_check_launch("pp_prefix_attention");
   if (rc != PP_OK) return rc;
-  PP_LAUNCH((prefix_join_kernel<Tile>), dim3(pp_blocks_1d((int64_t)a.B * a.L * a.H * (a.D / 4))), dim3(256), 0, stream, a);
+  constexpr int DL = Tile::kDB <= 1 ? 8 : Tile::kDB <= 2 ? 16 : Tile::kDB <= 4 ? 32 : 64;
+  int pg = 0;  // a part group gets up to 4 parts before there is another
+  while ((4 << pg) < a.parts && (2 << pg) * DL <= 256) ++pg;
+  const int64_t per = 256 / (DL << pg), blocks = ((int64_t)a.B * a.L * a.H + per - 1) / per;
+  if (blocks * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the join needs 2^32 threads or more");
+  PP_LAUNCH((prefix_join_kernel<Tile, DL>), dim3((unsigned)blocks), dim3(256), 0, stream, a, pg);
   return pp_check_launch("pp_prefix_attention(join)");
 }
 

@@ -288,7 +288,7 @@ struct AttnTile<float, DP, RB_, NS_> {
   typedef float type;
   static_assert(RB_ == 1 && NS_ == 1, "f32: one row block, 32 keys a step");
   static constexpr int RB = 1, NS = 1, kBN = 32, kRows = 128;
-  static constexpr int kWaves = DP > 64 ? 1 : 2;  // per SIMD
+  static constexpr int kWaves = DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kP = DP + 4;
   static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + 255) / 256, kDB = DP / 32, kQF = DP / 8;
   static constexpr int kSlot = kBN * kP, kFlag = 4 * kSlot * 4, kSmem = kFlag + 16;

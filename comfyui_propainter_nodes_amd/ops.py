@@ -1194,11 +1194,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
 
 
 def prefix_splits(b: int, new: int, p: int, s: int, h: int, kh: int) -> tuple[int, int]:
-    """(pieces of the prefix, pieces of an own range) of a prefix_attention call."""
+    """(pieces of the prefix, pieces of an own range) of a prefix_attention call: pieces of about the same length, a multiple of 64 keys, that
+    together make the 512 work-groups that the chip holds at once (two per CU)."""
     tiles = -(-b * new * (h // kh) // 128) * kh
-    own = -(-new * (h // kh) // 128) * kh * b
-    # 512 work-groups fill the chip twice over; a piece has at least 256 keys
-    return (max(1, min(-(-p // 256), 512 // max(1, tiles))) if p else 0), (max(1, min(-(-s // 256), 512 // max(1, own))) if s else 0)
+    own = -(-new * (h // kh) // 128) * kh * b if s else 0
+    piece = max(64, -(-(tiles * p + own * s) // (512 * 64)) * 64)
+    return -(-p // piece), -(-s // piece)
 
 
 def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_own: torch.Tensor, v_own: torch.Tensor,
