@@ -29,7 +29,7 @@ struct PrefixK {
 };
 
 template <typename Tile>
-__global__ void __launch_bounds__(256, Tile::kWaves) prefix_attention_kernel(const PrefixK a) {
+__global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention_kernel(const PrefixK a) {
   typedef typename Tile::type T;
   constexpr int kRows = Tile::kRows, RB = Tile::RB;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
@@ -191,7 +191,7 @@ static int launch_prefix(void* stream, pp::PrefixK& a) {
   const int64_t items = a.prefix_items + (int64_t)a.own_splits * a.B * a.own_tiles * a.KH;
   if (items * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the launch needs 2^32 threads or more");
   PP_ALLOW_BIG_LDS((&prefix_attention_kernel<Tile>), Tile::kSmem);
-  if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(256), Tile::kSmem, stream, a);
+  if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(Tile::kThreads), Tile::kSmem, stream, a);
   const int rc = pp_check_launch("pp_prefix_attention");
   if (rc != PP_OK) return rc;
   constexpr int DL = Tile::kDB <= 1 ? 8 : Tile::kDB <= 2 ? 16 : Tile::kDB <= 4 ? 32 : 64;
@@ -207,22 +207,18 @@ template <typename T>
 static int launch_prefix_d(void* stream, pp::PrefixK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
-    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 2>>(stream, a);
-#ifdef RB2
-    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 2, 2>>(stream, a);
-#elif defined(NS1)
-    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 1>>(stream, a);
-#endif
-    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 2>>(stream, a);
+    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 1, 2>>(stream, a);
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 1, 2>>(stream, a);
+    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1, 1>>(stream, a);
+    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1, 1>>(stream, a);
+    return launch_prefix<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+  } else {
+    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 1, 1>>(stream, a);
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 1, 1>>(stream, a);
+    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1, 1>>(stream, a);
+    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1, 1>>(stream, a);
+    return launch_prefix<AttnTile<T, 256, 4, 1, 1>>(stream, a);
   }
-  if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 1, 1>>(stream, a);
-  if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 1, 1>>(stream, a);
-  if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 1, 1>>(stream, a);
-#ifdef RB2
-  if constexpr (sizeof(T) == 2) if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 2, 1>>(stream, a);
-#endif
-  if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 1, 1>>(stream, a);
-  return launch_prefix<AttnTile<T, 256, 1, 1>>(stream, a);
 }
 
 extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_params* p) {

@@ -32,7 +32,7 @@ __device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
 }
 
 template <typename Tile>
-__global__ void __launch_bounds__(256, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
+__global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
   typedef typename Tile::type T;
   constexpr int kRows = Tile::kRows, RB = Tile::RB;
   const int kh = (int)blockIdx.x % a.KH;
@@ -107,7 +107,7 @@ static int launch_prompt(void* stream, pp::PromptK& a) {
   if (ntiles * a.KH * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
   a.ntiles = (int)ntiles;
   PP_ALLOW_BIG_LDS((&prompt_attention_kernel<Tile>), Tile::kSmem);
-  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH)), dim3(256), Tile::kSmem, stream, a);
+  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
   return pp_check_launch("pp_prompt_attention");
 }
 
@@ -115,22 +115,26 @@ template <typename T>
 static int launch_prompt_d(void* stream, pp::PromptK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
-    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 2>>(stream, a);
-#ifdef RB2
-    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 2>>(stream, a);
-#elif defined(NS1)
-    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 1>>(stream, a);
-#endif
-    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 2>>(stream, a);
+    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 1, 2>>(stream, a);
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 1, 2>>(stream, a);
+    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1, 1>>(stream, a);
+    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1, 1>>(stream, a);
+    return launch_prompt<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+  } else {
+    // Rows of a sequence that fit one 64-row work-group of 2 waves: with 4 waves half of them would idle (45 rows and keys, 128 channels: 153
+    // -> 133 us for 2592 sequences and heads).  Long sequences share the staging of 4 waves (2048 tokens: 277 us against 424).
+    if (a.Tq * a.G <= 64 * (int64_t)a.B) {
+      if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 2, 1, 1>>(stream, a);
+      if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 1, 1>>(stream, a);
+      if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 2, 1, 1>>(stream, a);
+      if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 2, 1, 1>>(stream, a);
+    }
+    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 1, 1>>(stream, a);
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 1, 1>>(stream, a);
+    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1, 1>>(stream, a);
+    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1, 1>>(stream, a);
+    return launch_prompt<AttnTile<T, 256, 4, 1, 1>>(stream, a);
   }
-  if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 1, 1>>(stream, a);
-  if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 1, 1>>(stream, a);
-  if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 1, 1>>(stream, a);
-#ifdef RB2
-  if constexpr (sizeof(T) == 2) if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 2, 1>>(stream, a);
-#endif
-  if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 1, 1>>(stream, a);
-  return launch_prompt<AttnTile<T, 256, 1, 1>>(stream, a);
 }
 
 extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p) {

@@ -1,6 +1,6 @@
 // tile_attention.h -- one work-group's attention over a run of keys: the part that pp_prompt_attention and pp_prefix_attention share.
 //
-// A work-group of 4 waves takes 128 RB query rows, 32 RB per wave, of ONE key / value head (the query heads of a group are rows of the
+// A work-group of NW waves takes 32 RB NW query rows, 32 RB per wave, of ONE key / value head (the query heads of a group are rows of the
 // same tile, so their keys are staged once).  Keys are walked in steps of 32 NS through LDS:
 //   S^T = K . Q^T     32x32 MFMA; lane l holds the scores of query l & 31 against keys (r & 3) + 8 (r >> 2) + 4 (l >> 5), r = 0..15
 //   online softmax    lane-local, one exchange between lanes l and l ^ 32; fp32 maxima, sums and accumulators
@@ -37,11 +37,17 @@ __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
 #ifdef PP_EMU
 inline void keep_branch() {}
+template <int N>
+inline void wave_priority() {}
 inline void pin(float&) {}
 inline void pin(unsigned&) {}
 #else
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }  // the value is computed by here
 __device__ __forceinline__ void pin(unsigned& v) { asm volatile("" : "+v"(v)); }
+template <int N>
+__device__ __forceinline__ void wave_priority() {
+  __builtin_amdgcn_s_setprio(N);
+}
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }  // what follows is not computed ahead of its condition
 #endif
 // A block of rows that is read 16 bytes at a time; what starts behind its last byte reads as zeros.  The base is wave-uniform, a lane's
@@ -116,13 +122,14 @@ __device__ __forceinline__ int score_key(int r, int h) { return (r & 3) + 8 * (r
 // 16-bit storage.  The two K and two V slots of 32 NS keys lie in LDS row by row, kPitch bytes a row, their 16-byte pieces XOR-swizzled so
 // that the K reads (16 bytes of 32 rows at once) and the transposing V reads (64 bytes of 4 rows at once) touch every bank once.
 // ----------------------------------------------------------------------------------------
-template <typename T, int DP, int RB_, int NS_>
+template <typename T, int DP, int NW_, int RB_, int NS_>
 struct AttnTile {
   typedef T type;
-  static constexpr int RB = RB_, NS = NS_, kBN = 32 * NS, kRows = 128 * RB;
+  static constexpr int NW = NW_, RB = RB_, NS = NS_, kThreads = 64 * NW, kBN = 32 * NS, kRows = 32 * NW * RB;
+  static constexpr bool kSteady = true;  // has products(): the pipelined step
   static constexpr int kWaves = RB > 1 || DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kPitch = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
-  static constexpr int kPieces = DP / 8, kPer = 8, kAll = kBN * kPieces, kStage = (kAll + 255) / 256, kDB = DP / 32, kQF = DP / 16;
+  static constexpr int kPieces = DP / 8, kPer = 8, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 16;
   static constexpr int kSlot = kBN * kPitch, kFlag = 4 * kSlot, kSmem = kFlag + 16;
   struct P {
     h8 f[2];
@@ -193,9 +200,11 @@ struct AttnTile {
     const h4 hi = lds_read_tr16(reinterpret_cast<const half_t*>(smem + v_at(slot, row + 8, piece) + (i & 1) * 8));
     return h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
-  __device__ __forceinline__ void pv(int slot, const P (*p)[NS], f16v (*o)[kDB]) const {
+  // keys: wave-uniform; sub-tiles behind the last one that any row sees are left out
+  __device__ __forceinline__ void pv(int slot, const P (*p)[NS], f16v (*o)[kDB], int keys) const {
 #pragma unroll
-    for (int sub = 0; sub < NS; ++sub)
+    for (int sub = 0; sub < NS; ++sub) {
+      if (sub > 0 && 32 * sub >= keys) break;
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -204,6 +213,7 @@ struct AttnTile {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) o[rb][db] = Op<T>::mfma(a, p[rb][sub].f[m], o[rb][db]);
         }
+    }
   }
   // A whole step: w = K Q^T, o += V^T z, y = exp2(x sc + nm) with its sums in bs.  The MFMAs are laid out one fragment at a time, each
   // followed by its share of the exponentials, and the LDS reads run kAhead fragments ahead: left to itself the compiler puts all the vector
@@ -283,14 +293,15 @@ struct AttnTile {
 // f32 storage: both products on v_mfma_f32_32x32x2_f32 (64 cycles for 2 keys or channels: the matrix pipe is the bound by far, LDS and
 // the vector ALU have slack).  Rows have a pitch of DP + 4 floats.
 // ----------------------------------------------------------------------------------------
-template <int DP, int RB_, int NS_>
-struct AttnTile<float, DP, RB_, NS_> {
+template <int DP, int NW_, int RB_, int NS_>
+struct AttnTile<float, DP, NW_, RB_, NS_> {
   typedef float type;
   static_assert(RB_ == 1 && NS_ == 1, "f32: one row block, 32 keys a step");
-  static constexpr int RB = 1, NS = 1, kBN = 32, kRows = 128;
+  static constexpr int NW = NW_, RB = 1, NS = 1, kThreads = 64 * NW, kBN = 32, kRows = 32 * NW;
+  static constexpr bool kSteady = false;  // (the vector work is a twentieth of the matrix work: nothing to overlap by hand)
   static constexpr int kWaves = DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kP = DP + 4;
-  static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + 255) / 256, kDB = DP / 32, kQF = DP / 8;
+  static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 8;
   static constexpr int kSlot = kBN * kP, kFlag = 4 * kSlot * 4, kSmem = kFlag + 16;
   struct P {
     float f[16];
@@ -338,22 +349,16 @@ struct AttnTile<float, DP, RB_, NS_> {
     return f;
   }
   __device__ __forceinline__ float v_val(int slot, int r, int db) const { return smem[(2 + slot) * kSlot + score_key(r, h) * kP + 32 * db + q32]; }
-  __device__ __forceinline__ void pv(int slot, const P (*p)[1], f16v (*o)[kDB]) const {
+  // keys: wave-uniform; groups of 8 keys behind the last one that any row sees are left out
+  __device__ __forceinline__ void pv(int slot, const P (*p)[1], f16v (*o)[kDB], int keys) const {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int g = 0; g < 4; ++g)
+      if (8 * g < keys) {
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
-  }
-  __device__ __forceinline__ void products(int slot, f16v (&w)[1][1], const P (&z)[1][1], f16v (*o)[kDB], const f16v (&x)[1][1],
-                                           P (&y)[1][1], const float* nm, float sc, float* bs) const {
-    qk(slot, w);
-    bs[0] = 0.f;
+        for (int r = 4 * g; r < 4 * g + 4; ++r)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      y[0][0].f[r] = fast_exp2(__builtin_fmaf(x[0][0][r], sc, nm[0]));
-      bs[0] += y[0][0].f[r];
-    }
-    pv(slot, z, o);
+          for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
+      }
   }
   static __device__ __forceinline__ bool scrub(u4& w) {
     bool any = false;
@@ -411,7 +416,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   unsigned koff[Tile::kStage], voff[Tile::kStage];
 #pragma unroll
   for (int i = 0; i < Tile::kStage; ++i) {
-    const int at = (int)threadIdx.x + 256 * i, row = at / Tile::kPieces, piece = at - row * Tile::kPieces;
+    const int at = (int)threadIdx.x + Tile::kThreads * i, row = at / Tile::kPieces, piece = at - row * Tile::kPieces;
     const bool in = piece * Tile::kPer < D && row < BN;
     koff[i] = in ? (unsigned)(row * k_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
     voff[i] = in ? (unsigned)(row * v_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
@@ -436,15 +441,15 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   auto store_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < Tile::kStage; ++j) {
-      const int at = (int)threadIdx.x + 256 * j, row = at / Tile::kPieces;
-      if (Tile::kAll % 256 == 0 || at < Tile::kAll) t.store_k(slot, j, row, at - row * Tile::kPieces);
+      const int at = (int)threadIdx.x + Tile::kThreads * j, row = at / Tile::kPieces;
+      if (Tile::kAll % Tile::kThreads == 0 || at < Tile::kAll) t.store_k(slot, j, row, at - row * Tile::kPieces);
     }
   };
   auto store_v = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < Tile::kStage; ++j) {
-      const int at = (int)threadIdx.x + 256 * j, row = at / Tile::kPieces;
-      if (Tile::kAll % 256 == 0 || at < Tile::kAll) t.store_v(slot, j, row, at - row * Tile::kPieces);
+      const int at = (int)threadIdx.x + Tile::kThreads * j, row = at / Tile::kPieces;
+      if (Tile::kAll % Tile::kThreads == 0 || at < Tile::kAll) t.store_v(slot, j, row, at - row * Tile::kPieces);
     }
   };
 
@@ -457,6 +462,25 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   float nm[RB], bs[RB];  // -m sc (NaN before the first visible key: whatever a block holds, it is taken again); sums over the block
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) nm[rb] = __builtin_nanf("");
+  auto softmax = [&](const Scores& x, Probs& y) __attribute__((always_inline)) -> bool {  // x -> y, bs; did a sum come out too large?
+    bool over = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      bs[rb] = 0.f;
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) {
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+          bs[rb] += e[r];
+        }
+        y[rb][sub] = Tile::pack_p(e);
+      }
+      over |= !(bs[rb] <= kMost);
+    }
+    return wave_any(over);
+  };
   // moves the maximum to that of x and what was summed up with it; x -> y, bs
   auto move_max = [&](const Scores& x, Probs& y) __attribute__((always_inline)) {
     keep_branch();
@@ -498,11 +522,14 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   };
   // softmax of block i (x -> y), second product of block i - 1 (z), first product of block i + 1 (-> w); every live row of the work-group
   // sees all of block i
-  auto fast_step = [&](int i, auto slot, const Scores& x, Scores& w, const Probs& z, Probs& y) __attribute__((always_inline)) {
+  [[maybe_unused]] auto fast_step = [&](int i, auto slot, const Scores& x, Scores& w, const Probs& z, Probs& y) __attribute__((always_inline)) {
     constexpr int S0 = decltype(slot)::value, S1 = 1 - S0;
     stage(i, S0);
     if (lim.wave_max > 0) {
-      t.products(S1, w, z, st.o, x, y, nm, sc, bs);
+      // a wave that is in its products goes before one that stages (D = 128: 533 -> 530 us, 507 -> 498 without a mask; 64: 330 -> 334, so not there)
+      if constexpr (Tile::kDB > 2) wave_priority<1>();
+      if constexpr (Tile::kSteady) t.products(S1, w, z, st.o, x, y, nm, sc, bs);
+      if constexpr (Tile::kDB > 2) wave_priority<0>();
       bool over = false;
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) over |= !(bs[rb] <= kMost);
@@ -521,7 +548,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
         if (Tile::scrub(t.vs[j])) *flag = 1;
     }
     stage(i, s0);
-    if (i > 0 && (i - 1) * BN < lim.wave_max) t.pv(s1, p, st.o);
+    if (i > 0 && (i - 1) * BN < lim.wave_max) t.pv(s1, p, st.o, lim.wave_max - (i - 1) * BN);
     if (i * BN < lim.wave_max) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -531,7 +558,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
         }
-      move_max(s, p);
+      if (softmax(s, p)) move_max(s, p);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) st.l[rb] += bs[rb];
       if ((i + 1) * BN < lim.wave_max) t.qk(s1, s);
@@ -561,13 +588,15 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   const int nfast = mixed_from / BN;
   for (int i = 0; i < nsteps;) {
     any_step(i);
-    if (++i == 1)
-      for (; i + 2 <= nfast; i += 2) {
-        fast_step(i, std::integral_constant<int, 1>{}, s, s2, p, p2);
-        fast_step(i + 1, std::integral_constant<int, 0>{}, s2, s, p2, p);
-      }
+    ++i;
+    if constexpr (Tile::kSteady)
+      if (i == 1)
+        for (; i + 2 <= nfast; i += 2) {
+          fast_step(i, std::integral_constant<int, 1>{}, s, s2, p, p2);
+          fast_step(i + 1, std::integral_constant<int, 0>{}, s2, s, p2, p);
+        }
   }
-  if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o);
+  if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o, lim.wave_max - (nsteps - 1) * BN);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) st.l[rb] = pair32_sum(st.l[rb]);
   st.not_finite = *flag != 0;

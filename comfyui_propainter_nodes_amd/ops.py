@@ -39,6 +39,7 @@ EPI = {
 }
 # activations of groupnorm (the convolutions' epilogues know all of them but silu)
 NORM_ACT = {**ACT, "silu": _lib.CONSTS["PP_ACT_SILU"]}
+_GROUPNORM, _PROMPT, _PREFIX = (_lib.packer(f"pp_{n}_params") for n in ("groupnorm", "prompt_attention", "prefix_attention"))
 _LM_DTYPE = {torch.float32: PP_F32, torch.float16: PP_F16, torch.bfloat16: _lib.CONSTS["PP_BF16"]}
 PAD = {"zeros": _lib.CONSTS["PP_PAD_ZEROS"], "replicate": _lib.CONSTS["PP_PAD_REPLICATE"]}
 
@@ -159,22 +160,27 @@ def stream_handle(t: torch.Tensor) -> int:
 def check_device(*tensors: torch.Tensor) -> None:
     """The gfx950 library takes device pointers only; the emulator (tests) takes host pointers."""
     L = _lib.current()
+    current = None
     for t in tensors:
         if t is None:
             continue
+        at = t.get_device()      # -1: host memory
         if L.is_emulator:
             if t.is_cuda:
                 raise RuntimeError("emulator library loaded but a CUDA tensor was passed")
-        elif not t.is_cuda:
+        elif at < 0 or not t.is_cuda:
             raise RuntimeError(
                 "libpropainter_mi355 needs tensors on the MI355X (got a CPU tensor); there is no CPU fallback"
             )
-        elif t.device.index != torch.cuda.current_device():
-            # hipLaunchKernel resolves the kernel for the CURRENT device: launching onto a stream of another device is undefined.
-            # A process that drives several GPUs makes the tensor's device current first (distributed.run_multi_device: one thread
-            # per device; `with torch.cuda.device(d)` elsewhere).
-            raise RuntimeError(f"tensor on {t.device} but the current HIP device is cuda:{torch.cuda.current_device()}: "
-                               "make the tensor's device current before calling libpropainter_mi355")
+        else:
+            if current is None:
+                current = torch.cuda.current_device()
+            if at != current:
+                # hipLaunchKernel resolves the kernel for the CURRENT device: launching onto a stream of another device is undefined.
+                # A process that drives several GPUs makes the tensor's device current first (distributed.run_multi_device: one thread
+                # per device; `with torch.cuda.device(d)` elsewhere).
+                raise RuntimeError(f"tensor on {t.device} but the current HIP device is cuda:{current}: "
+                                   "make the tensor's device current before calling libpropainter_mi355")
 
 
 def nhwc_view(t: torch.Tensor) -> tuple[int, int, int, int, int]:
@@ -677,13 +683,15 @@ def groupnorm(x: torch.Tensor, y: torch.Tensor, groups: int, gamma: torch.Tensor
     n, h, w, c, x_ldc = nhwc_view(x)
     if y.shape != x.shape or (skip is not None and skip.shape != x.shape):
         raise ValueError("groupnorm: x, y and skip must share a shape")
+    y_ldc = nhwc_view(y)[4]
     code = _lm_dtype("groupnorm", x, y, skip)
     if groups < 1 or c % groups:
         raise ValueError(f"groupnorm: {c} channels are not a multiple of {groups} groups")
     for name, t in (("gamma", gamma), ("beta", beta)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous()):
             raise ValueError(f"groupnorm: {name} must be a dense fp32 [{c}] tensor")
-    if act not in NORM_ACT:
+    act_code = NORM_ACT.get(act)
+    if act_code is None:
         raise ValueError(f"groupnorm: unknown activation {act!r}")
     need, nchunks = groupnorm_scratch(n, h * w, c, groups, x.element_size())
     if scratch is None:
@@ -692,17 +700,12 @@ def groupnorm(x: torch.Tensor, y: torch.Tensor, groups: int, gamma: torch.Tensor
         check_device(scratch)
         if scratch.dtype != torch.float64 or scratch.numel() < need or not scratch.is_contiguous():
             raise ValueError(f"groupnorm: scratch must be a dense float64 tensor of at least {need} elements")
-    P = _lib.STRUCTS["pp_groupnorm_params"]()
-    P.dtype, P.act, P.act_param, P.relu_post, P.eps = code, NORM_ACT[act], act_param, int(relu_post), eps
-    P.x, P.x_ldc, P.y, P.y_ldc = x.data_ptr(), x_ldc, y.data_ptr(), nhwc_view(y)[4]
-    if skip is not None:
-        P.skip, P.skip_ldc = skip.data_ptr(), nhwc_view(skip)[4]
-    P.gamma = gamma.data_ptr() if gamma is not None else None
-    P.beta = beta.data_ptr() if beta is not None else None
-    P.N, P.HW, P.C, P.groups = n, h * w, c, groups
-    P.partials, P.nchunks = scratch.data_ptr(), nchunks
     if n * h * w > 0:
-        _call("pp_groupnorm", y, P)
+        _lib.current().call_packed("pp_groupnorm", stream_handle(y), _GROUPNORM.pack(
+            code, act_code, x.data_ptr(), x_ldc, y.data_ptr(), y_ldc,
+            0 if skip is None else skip.data_ptr(), 0 if skip is None else nhwc_view(skip)[4],
+            0 if gamma is None else gamma.data_ptr(), 0 if beta is None else beta.data_ptr(),
+            n, h * w, c, groups, scratch.data_ptr(), nchunks, eps, act_param, int(relu_post)))
     return y
 
 
@@ -1142,16 +1145,19 @@ def window_attention(qkv: torch.Tensor, pkv: torch.Tensor, win_masked: torch.Ten
 
 def _heads_view(name: str, t: torch.Tensor, dims: int) -> tuple:
     """Element strides of a [..., heads, D] view (0 for dims of one element, whose stride says nothing)."""
-    if t.dim() != dims:
-        raise ValueError(f"{name}: expected {dims} dims, got {tuple(t.shape)}")
     st, sh = t.stride(), t.shape
+    if len(st) != dims:
+        raise ValueError(f"{name}: expected {dims} dims, got {tuple(sh)}")
     if st[-1] != 1 and sh[-1] > 1:
         raise ValueError(f"{name}: the last dim must be dense, got strides {st}")
-    return tuple(a if n > 1 else 0 for a, n in zip(st[:-1], sh[:-1]))
+    if 1 in sh:
+        return tuple(a if n > 1 else 0 for a, n in zip(st[:-1], sh[:-1]))
+    return st[:-1]
 
 
 def _writable(name: str, t: torch.Tensor) -> None:
-    if any(a == 0 and n > 1 for a, n in zip(t.stride(), t.shape)):
+    st = t.stride()
+    if 0 in st and any(a == 0 and n > 1 for a, n in zip(st, t.shape)):
         raise ValueError(f"{name}: an expanded view cannot be written")
 
 
@@ -1177,19 +1183,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
             raise ValueError(f"prompt_attention: {name} must be a dense int32 [sequences + 1] tensor")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tq, h) or not lse.is_contiguous()):
         raise ValueError(f"prompt_attention: lse must be a dense fp32 [{tq}, {h}] tensor")
-    P = _lib.STRUCTS["pp_prompt_attention_params"]()
-    P.dtype, P.causal, P.scale = code, int(causal), d ** -0.5 if scale is None else scale
-    P.q, P.q_row, P.q_head = q.data_ptr(), qs[0], qs[1]
-    P.k, P.k_row, P.k_head = k.data_ptr(), ks[0], ks[1]
-    P.v, P.v_row, P.v_head = v.data_ptr(), vs[0], vs[1]
-    P.out, P.out_row, P.out_head = out.data_ptr(), os_[0], os_[1]
-    P.lse = lse.data_ptr() if lse is not None else None
-    P.cu_q, P.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
-    P.B, P.Tq, P.Tk, P.H, P.KH, P.D = cu_q.numel() - 1, tq, tk, h, kh, d
     if tq > 0:
-        if tk == 0:          # every row is empty; an empty tensor has no address
-            P.k = P.v = P.q
-        _call("pp_prompt_attention", out, P)
+        qp = q.data_ptr()
+        _lib.current().call_packed("pp_prompt_attention", stream_handle(out), _PROMPT.pack(
+            code, int(causal), qp, *qs, k.data_ptr() if tk else qp, *ks, v.data_ptr() if tk else qp, *vs, out.data_ptr(), *os_,
+            0 if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, tq, tk, h, kh, d,
+            d ** -0.5 if scale is None else scale))      # (tk = 0: every row is empty; an empty tensor has no address)
     return out
 
 
@@ -1230,28 +1229,20 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     if own_len.dtype != torch.int32 or own_len.shape != (b,) or not own_len.is_contiguous():
         raise ValueError(f"prefix_attention: own_len must be a dense int32 [{b}] tensor")
     ps, osp = prefix_splits(b, new, p, s, h, kh)
-    need = prefix_attention_scratch(q, k_prefix, k_own)
+    if ps + osp == 0:
+        ps = 1
+    need = max(4, b * new * h * (ps + osp) * (d + 4))
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     else:
         check_device(scratch)
         if scratch.dtype != torch.float32 or scratch.numel() < need or not scratch.is_contiguous():
             raise ValueError(f"prefix_attention: scratch must be a dense float32 tensor of at least {need} elements")
-    P = _lib.STRUCTS["pp_prefix_attention_params"]()
-    P.dtype, P.prefix_splits, P.own_splits, P.scale = code, ps, osp, d ** -0.5 if scale is None else scale
-    if ps + osp == 0:
-        P.prefix_splits = 1
-    P.q, P.q_seq, P.q_row, P.q_head = q.data_ptr(), *qs
-    P.kp, P.kp_row, P.kp_head = k_prefix.data_ptr(), *kps
-    P.vp, P.vp_row, P.vp_head = v_prefix.data_ptr(), *vps
-    P.ko, P.ko_seq, P.ko_row, P.ko_head = k_own.data_ptr(), *kos
-    P.vo, P.vo_seq, P.vo_row, P.vo_head = v_own.data_ptr(), *vos
-    P.own_len = own_len.data_ptr()
-    P.out, P.out_seq, P.out_row, P.out_head = out.data_ptr(), *os_
-    P.scratch, P.scratch_bytes = scratch.data_ptr(), scratch.numel() * 4
-    P.B, P.L, P.P, P.S, P.H, P.KH, P.D = b, new, p, s, h, kh, d
     if b * new > 0:
-        _call("pp_prefix_attention", out, P)
+        _lib.current().call_packed("pp_prefix_attention", stream_handle(out), _PREFIX.pack(
+            code, ps, osp, d ** -0.5 if scale is None else scale, q.data_ptr(), *qs, k_prefix.data_ptr(), *kps, v_prefix.data_ptr(), *vps,
+            k_own.data_ptr(), *kos, v_own.data_ptr(), *vos, own_len.data_ptr(), out.data_ptr(), *os_, scratch.data_ptr(),
+            scratch.numel() * 4, b, new, p, s, h, kh, d))
     return out
 
 
