@@ -44,7 +44,7 @@ def _fold_bn(w, b, p, name):
 
 
 class _Encoder:
-    """BasicEncoder (extractor.py:121-193) as a list of conv specs; `kind` = instance | batch."""
+    """BasicEncoder (extractor.py:121-193) as a list of conv specs; `kind` = instance | batch | group (8 channels a group)."""
 
     def __init__(self, p: dict, kind: str, device):
         self.kind = kind
@@ -56,7 +56,15 @@ class _Encoder:
                 w, b = _fold_bn(w, b, p, norm)
             return w, b, kw
 
+        def affine(name):       # (gamma, beta) of a group norm
+            if kind != "group":
+                return None
+            return p[name + ".weight"].float().to(device), p[name + ".bias"].float().to(device)
+
+        if kind not in ("instance", "batch", "group"):
+            raise ValueError(f"encoder norm {kind!r}: instance, batch or group")
         w, b, _ = conv("conv1", "norm1")
+        self.n1 = affine("norm1")
         # 7x7 s2 on 3 channels -> im2col (k = (ky,kx,c)) + GEMM
         self.c1_kpad = ops.pad32(147)
         self.conv1 = _conv_spec(w.permute(0, 2, 3, 1).reshape(64, 147, 1, 1), b, dt, seg_channels=[self.c1_kpad],
@@ -71,11 +79,12 @@ class _Encoder:
                 blk = {
                     "c1": _conv_spec(w1, b1, dt, stride=st, padding=1).to(device),
                     "c2": _conv_spec(w2, b2, dt, padding=1).to(device),
-                    "down": None, "dim": dim, "stride": st,
+                    "down": None, "dim": dim, "stride": st, "n1": affine(pre + "norm1"), "n2": affine(pre + "norm2"), "n3": None,
                 }
                 if st != 1:
                     wd, bd, _ = conv(pre + "downsample.0", pre + "norm3")
                     blk["down"] = _conv_spec(wd, bd, dt, stride=st).to(device)
+                    blk["n3"] = affine(pre + "norm3")
                 self.blocks.append(blk)
                 cin = dim
         self.conv2 = _conv_spec(p["conv2.weight"], p["conv2.bias"], dt).to(device)
@@ -84,7 +93,14 @@ class _Encoder:
         """frames [n,H,W,3] fp32 -> out [n,H/8,W/8,256]."""
         dev = frames.device
         n, H, W, _ = frames.shape
-        inst = self.kind == "instance"
+        inst = self.kind != "batch"      # a norm of its own behind every convolution (a batch norm is folded into it)
+
+        def norm(y, affine, relu=True, skip=None):
+            """relu(norm(y)), norm(y), or relu(skip + relu(norm(y))), in place."""
+            if affine is None:
+                return ops.instnorm(y, y, relu_pre=relu, skip=skip, relu_post=skip is not None)
+            return ops.groupnorm(y, y, y.shape[3] // 8, *affine, act="relu" if relu else None, skip=skip, relu_post=skip is not None)
+
         h2, w2 = (H + 6 - 7) // 2 + 1, (W + 6 - 7) // 2 + 1
         x = torch.empty(n, h2, w2, 64, device=dev)
         if self.conv1.split and ops.patch_conv_enabled():
@@ -96,7 +112,7 @@ class _Encoder:
             ops.conv2d(self.conv1, [cols], x, act=None if inst else "relu")
             del cols
         if inst:
-            ops.instnorm(x, x, relu_pre=True)
+            norm(x, self.n1)
         for blk in self.blocks:
             _, h, w, _ = x.shape
             ho, wo = blk["c1"].out_hw(h, w)
@@ -104,14 +120,14 @@ class _Encoder:
             y2 = torch.empty(n, ho, wo, blk["dim"], device=dev)
             if inst:
                 ops.conv2d(blk["c1"], [x], y1)
-                ops.instnorm(y1, y1, relu_pre=True)
+                norm(y1, blk["n1"])
                 ops.conv2d(blk["c2"], [y1], y2)
                 skip = x
                 if blk["down"] is not None:
                     skip = torch.empty(n, ho, wo, blk["dim"], device=dev)
                     ops.conv2d(blk["down"], [x], skip)
-                    ops.instnorm(skip, skip)
-                ops.instnorm(y2, y2, relu_pre=True, skip=skip, relu_post=True)
+                    norm(skip, blk["n3"], relu=False)
+                norm(y2, blk["n2"], skip=skip)
             else:
                 ops.conv2d(blk["c1"], [x], y1, act="relu")
                 skip = x
@@ -128,7 +144,9 @@ class _Encoder:
 
 
 class RaftFlow:
-    def __init__(self, sd: dict, device, *, max_volume_bytes: int = 48 << 30, enc_chunk: int = 16):
+    def __init__(self, sd: dict, device, *, max_volume_bytes: int = 48 << 30, enc_chunk: int = 16, fnet_norm: str = "instance",
+                 cnet_norm: str = "batch"):
+        """fnet_norm / cnet_norm: the encoders' norm_fn (instance | batch | group); raft-things has the defaults."""
         self.device = torch.device(device)
         self.max_volume_bytes = max_volume_bytes
         self.enc_chunk = enc_chunk
@@ -136,8 +154,8 @@ class RaftFlow:
         self._ws: dict = {}       # per clip shape: the update graphs' static inputs (feature maps, per-pair context, tiled operand)
         self._side = None         # the second direction's stream
         dt = torch.float32
-        self.fnet = _Encoder(_strip(sd, "fnet."), "instance", device)
-        self.cnet = _Encoder(_strip(sd, "cnet."), "batch", device)
+        self.fnet = _Encoder(_strip(sd, "fnet."), fnet_norm, device)
+        self.cnet = _Encoder(_strip(sd, "cnet."), cnet_norm, device)
         u = _strip(sd, "update_block.")
 
         def spec(name, **kw):

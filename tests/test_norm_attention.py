@@ -458,3 +458,195 @@ def test_map_to_prompt_to_continuation(backend):
         tol = _attn_tol(F16, o, amp, 43, d, smax, all_v.abs().max().item())
         _within(step[i:i + 1], o, tol)
         _within(one, o, tol)
+
+
+# --------------------------------------------------------------------------------------------
+# the encoder that calls it
+# --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hw", [(40, 56)])
+def test_raft_encoder_with_group_norm(backend, hw):
+    """BasicEncoder(norm_fn="group"): 8 groups in the stem, planes // 8 in the blocks, against torch on the same weights.  The 16
+    convolutions run as two-term f16 splits (2^-20 of each operand) over at most 1152 products, the norms bring every map back to about
+    unit size, and nothing amplifies: 16 layers of 1152^0.5 * 2^-19 stay below 2e-3 of the largest output."""
+    from comfyui_propainter_nodes_amd import raft
+
+    g = torch.Generator().manual_seed(21)
+    p = {}
+
+    def conv(name, co, ci, k):
+        p[name + ".weight"] = torch.randn(co, ci, k, k, generator=g) * (ci * k * k) ** -0.5
+        p[name + ".bias"] = 0.1 * torch.randn(co, generator=g)
+
+    def affine(name, c):
+        p[name + ".weight"], p[name + ".bias"] = 1 + 0.2 * torch.randn(c, generator=g), 0.2 * torch.randn(c, generator=g)
+
+    conv("conv1", 64, 3, 7)
+    affine("norm1", 64)
+    ci = 64
+    for layer, dim, stride in (("layer1", 64, 1), ("layer2", 96, 2), ("layer3", 128, 2)):
+        for i, st in ((0, stride), (1, 1)):
+            pre = f"{layer}.{i}."
+            conv(pre + "conv1", dim, ci, 3)
+            conv(pre + "conv2", dim, dim, 3)
+            affine(pre + "norm1", dim)
+            affine(pre + "norm2", dim)
+            if st != 1:
+                conv(pre + "downsample.0", dim, ci, 1)
+                affine(pre + "norm3", dim)
+            ci = dim
+    conv("conv2", 256, 128, 1)
+    frames = torch.rand(2, *hw, 3, generator=g) * 2 - 1
+
+    def norm(x, name):
+        return F.group_norm(x, x.shape[1] // 8, p[name + ".weight"].double(), p[name + ".bias"].double(), 1e-5)
+
+    def cv(x, name, **kw):
+        return F.conv2d(x, p[name + ".weight"].double(), p[name + ".bias"].double(), **kw)
+
+    x = F.relu(norm(cv(frames.double().permute(0, 3, 1, 2), "conv1", stride=2, padding=3), "norm1"))
+    for layer, stride in (("layer1", 1), ("layer2", 2), ("layer3", 2)):
+        for i, st in ((0, stride), (1, 1)):
+            pre = f"{layer}.{i}."
+            y = F.relu(norm(cv(x, pre + "conv1", stride=st, padding=1), pre + "norm1"))
+            y = F.relu(norm(cv(y, pre + "conv2", padding=1), pre + "norm2"))
+            if st != 1:
+                x = norm(cv(x, pre + "downsample.0", stride=st), pre + "norm3")
+            x = F.relu(x + y)
+    ref = cv(x, "conv2").permute(0, 2, 3, 1)
+    enc = raft._Encoder(p, "group", backend)
+    out = torch.empty(2, hw[0] // 8, hw[1] // 8, 256, device=backend)
+    enc(frames.to(backend), out, split_tanh_relu=False)
+    assert (out.double().cpu() - ref).abs().max() <= 2e-3 * ref.abs().max()
+    with pytest.raises(ValueError, match="norm"):
+        raft._Encoder(p, "layer", backend)
+
+
+# --------------------------------------------------------------------------------------------
+# streams, graphs, sizes (MI355X)
+# --------------------------------------------------------------------------------------------
+def _calls(dev, seed):
+    """One call of each operator on inputs of its own -> (function, its outputs)."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(2, 24, 20, 320, generator=g).to(F16).to(dev)
+    y = torch.empty_like(x)
+    q, k, v = (torch.randn(90, n, 64, generator=g).to(BF16).to(dev) for n in (8, 2, 2))
+    out, cu = torch.empty_like(q), _cu([50, 0, 40], dev)
+    pq, ko, vo = torch.randn(3, 1, 8, 64, generator=g).to(BF16).to(dev), *(torch.randn(3, 70, 2, 64, generator=g).to(BF16).to(dev) for _ in range(2))
+    po, n = torch.empty_like(pq), torch.tensor([70, 1, 33], dtype=torch.int32, device=dev)
+
+    def run():
+        ops.groupnorm(x, y, 32, act="silu")
+        ops.prompt_attention(q, k, v, out, cu)
+        ops.prefix_attention(pq, k, v, ko, vo, n, po)
+
+    return run, (x, q, pq, ko), (y, out, po)
+
+
+@gpu_only
+def test_captured_and_replayed(hip_lib):
+    """Two graphs of the same operators, replayed in turn on changing inputs with eager calls between: every replay equals the eager result
+    bit for bit (no atomics, scratch of their own)."""
+    dev = torch.device("cuda:0")
+    both = [_calls(dev, s) for s in (31, 32)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for run, _, _ in both:
+            run()
+    side.synchronize()
+    graphs = []
+    for run, _, _ in both:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graphs.append(graph)
+    for rep in range(4):
+        for (run, ins, outs), graph in zip(both, graphs):
+            for t in ins:
+                t.mul_(0.9)
+            run()
+            want = [t.clone() for t in outs]
+            for t in outs:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(want, outs):
+                assert torch.equal(a, b), rep
+
+
+@gpu_only
+def test_two_streams_at_once(hip_lib):
+    dev = torch.device("cuda:0")
+    calls = [_calls(dev, s) for s in (41, 42)]
+    for run, _, _ in calls:
+        run()
+    torch.cuda.synchronize()
+    want = [[t.clone() for t in outs] for _, _, outs in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(10):
+        for st, (run, _, _) in zip(streams, calls):
+            with torch.cuda.stream(st):
+                run()
+    torch.cuda.synchronize()
+    for w, (_, _, outs) in zip(want, calls):
+        for a, b in zip(w, outs):
+            assert torch.equal(a, b)
+
+
+@gpu_only
+def test_long_and_wide(hip_lib):
+    """Key offsets past 2^32 elements, a long prompt, a long prefix: against f32 products of torch on a few rows."""
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(51)
+    kh, d, t = 2, 128, 700
+    big_k, big_v = (torch.empty(t, 1 << 23, dtype=F16, device=dev) for _ in range(2))      # 11.7 GB each: row 512 starts past 2^32
+    k, v = big_k[:, :kh * d].unflatten(1, (kh, d)), big_v[:, :kh * d].unflatten(1, (kh, d))
+    k.copy_(torch.randn(t, kh, d, device=dev, generator=g))
+    v.copy_(torch.randn(t, kh, d, device=dev, generator=g))
+    q = torch.randn(t, 8, d, device=dev, generator=g).to(F16)
+    out, same = torch.empty_like(q), torch.empty_like(q)
+    cu = _cu([t], dev)
+    ops.prompt_attention(q, k, v, out, cu)
+    ops.prompt_attention(q, k.contiguous(), v.contiguous(), same, cu)
+    assert torch.equal(out, same)
+    own_k, own_v = k[None, :1].contiguous(), v[None, :1].contiguous()
+    one = torch.empty(1, 8, d, dtype=F16, device=dev)
+    ops.prefix_attention(q[-1:], k, v, own_k, own_v, torch.zeros(1, dtype=torch.int32, device=dev), one)
+    tol = 4 * U[F16] * v.float().abs().max()
+    assert (one[0] - out[-1]).abs().max() <= tol         # the last token of the prompt sees the same keys
+    del big_k, big_v, k, v
+    torch.cuda.empty_cache()
+    n = 20000
+    q, k, v = (torch.randn(n, h, 64, device=dev, generator=g).to(BF16) for h in (4, 1, 1))
+    out = torch.empty_like(q)
+    ops.prompt_attention(q, k, v, out, _cu([n], dev))
+    for row in (0, 31, 32, 9999, n - 1):
+        o, amp, _, smax = _attend_ref(q[row:row + 1].double().cpu(), k[:row + 1].double().cpu(), v[:row + 1].double().cpu(),
+                                      torch.ones(1, row + 1, dtype=torch.bool), 64 ** -0.5)
+        _within(out[row:row + 1], o, _attn_tol(BF16, o, amp, row + 1, 64, smax, v.float().abs().max().item()), row)
+
+
+@gpu_only
+@DT
+@pytest.mark.parametrize("h,kh,d,lens,causal", [
+    (8, 2, 64, [1000, 3, 517], True), (4, 4, 128, [300, 290], False), (6, 2, 96, [257, 128, 129], True), (2, 1, 256, [200, 310], True),
+    (3, 1, 32, [700], True), (16, 1, 80, [100, 33], True)])
+def test_prompt_attention_through_the_steady_state(hip_lib, dt, h, kh, d, lens, causal):
+    """Sequences of many key blocks: the pipelined steps, both parities of their number, rising and falling maxima."""
+    _check_prompt(torch.device("cuda:0"), dt, h, kh, d, lens, lens, causal)
+
+
+@DT
+@pytest.mark.parametrize("rising", [True, False])
+def test_prompt_attention_with_moving_maxima(backend, dt, rising):
+    """Scores that rise (or fall) by hundreds along the keys: the maximum has to move (or stay) in every block."""
+    g = torch.Generator().manual_seed(61)
+    n, d = 230, 32
+    q = torch.randn(n, 1, d, generator=g) * 0.05 + 1
+    k = torch.randn(n, 1, d, generator=g) * 0.05 + (torch.arange(n) if rising else torch.arange(n).flip(0))[:, None, None] * 0.1
+    v = torch.randn(n, 1, d, generator=g)
+    q, k, v = (t.to(dt).to(backend) for t in (q, k, v))
+    for causal in (False, True):
+        out = torch.empty_like(q)
+        ops.prompt_attention(q, k, v, out, _cu([n], backend), causal=causal, scale=1.0)
+        o, amp, _, smax = _attend_ref(q.double().cpu(), k.double().cpu(), v.double().cpu(), _seen(n, n, causal), 1.0)
+        _within(out, o, _attn_tol(dt, o, amp, n, d, smax, v.float().abs().max().item()))
