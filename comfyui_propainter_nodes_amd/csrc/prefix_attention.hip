@@ -5,8 +5,7 @@
 // prefix of P keys is staged ceil(B L G / 128) times instead of B times, and the two products run at matrix speed.  The prefix is
 // cut into pieces so that few rows still fill the chip; the own keys of a sequence (its L G rows) are work-groups of the same launch.  Every piece
 // leaves (maximum, sum, sum of weighted values) in fp32; a second launch joins them in piece order.
-#include "tile_attention.h"
-#include "pp_host.h"
+#include "attention_parts.h"
 
 #include <math.h>
 
@@ -16,13 +15,11 @@ namespace pp {
 
 struct PrefixK {
   const void *q, *kp, *vp, *ko, *vo;
-  void* out;
   const int* own_len;
-  float* part_o;   // [row][part][D]
-  float* part_ml;  // [row][part][2]
-  int64_t q_seq, q_row, q_head, kp_row, kp_head, vp_row, vp_head, ko_seq, ko_row, ko_head, vo_seq, vo_row, vo_head, out_seq, out_row, out_head;
+  PartsK parts;
+  int64_t q_seq, q_row, q_head, kp_row, kp_head, vp_row, vp_head, ko_seq, ko_row, ko_head, vo_seq, vo_row, vo_head;
   int64_t P, S;
-  int B, L, H, KH, G, D, prefix_splits, own_splits, parts;
+  int B, L, H, KH, G, D, prefix_splits, own_splits;
   int prefix_tiles, own_tiles;  // 128-row tiles of all B L G rows / of one sequence's L G rows
   int64_t prefix_items;         // work-groups of the prefix part; those of the own part follow
   float sc;
@@ -101,82 +98,8 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
     if (row > last) continue;
     const int64_t b = shared ? row / lg : seq;
     const int in_seq = (int)(shared ? row % lg : row);
-    const int64_t at = ((b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G) * a.parts + part;
-    float* dst = a.part_o + at * a.D;
-#pragma unroll
-    for (int db = 0; db < Tile::kDB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * db + 8 * g + 4 * h;
-        const f16v& o = st.o[rb][db];
-        if (d < a.D) *reinterpret_cast<f4*>(dst + d) = f4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
-      }
-    if (h == 0) {
-      a.part_ml[2 * at] = st.m[rb];
-      a.part_ml[2 * at + 1] = st.l[rb];
-    }
+    store_part(a.parts, t, st, rb, (b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G, part, lim.row[rb] > 0);
   }
-}
-
-// Joins the parts of a row: a row's D values are DL threads of 4, and PG groups of such threads take every PG-th part each, four parts'
-// loads in flight; then the groups' results are joined in LDS.  (One thread per 4 values walking all parts took 17 us for 33 parts of 1024 rows.)
-template <typename Tile, int DL>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixK a, int pg_log2) {
-  typedef typename Tile::type T;
-  __shared__ f4 so[256];
-  __shared__ float sm[256], sl[256];
-  const int tid = (int)threadIdx.x, dl = tid % DL, PG = 1 << pg_log2, pg = tid / DL % PG, slot = tid / (DL * PG);
-  const int64_t row = (int64_t)blockIdx.x * (256 / (DL * PG)) + slot, rows = (int64_t)a.B * a.L * a.H;
-  const bool live = row < rows && 4 * dl < a.D;
-  float m = neg_inf(), l = 0.f;
-  f4 o = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    const float* ml = a.part_ml + row * a.parts * 2;
-    const float* po = a.part_o + row * a.parts * a.D + 4 * dl;
-    for (int p0 = pg; p0 < a.parts; p0 += 4 * PG) {
-      float pm[4], pl[4];
-      f4 v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int p = p0 + u * PG;
-        const bool in = p < a.parts;
-        pm[u] = in ? ml[2 * p] : neg_inf();
-        pl[u] = in ? ml[2 * p + 1] : 0.f;
-        v[u] = in ? *reinterpret_cast<const f4*>(po + (int64_t)p * a.D) : f4{0.f, 0.f, 0.f, 0.f};
-      }
-      const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
-      const float w = m == top ? 1.f : fast_exp2((m - top) * a.sc);
-      m = top;
-      l *= w;
-      o *= w;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float x = pm[u] == top ? 1.f : fast_exp2((pm[u] - top) * a.sc);
-        l += x * pl[u];
-        o += x * v[u];
-      }
-    }
-  }
-  so[tid] = o;
-  sm[tid] = m;
-  sl[tid] = l;
-  __syncthreads();
-  if (!live || pg != 0) return;
-  float top = m;
-  for (int g = 1; g < PG; ++g) top = fmaxf(top, sm[tid + g * DL]);
-  const float w = m == top ? 1.f : fast_exp2((m - top) * a.sc);
-  l *= w;
-  o *= w;
-  for (int g = 1; g < PG; ++g) {
-    const float x = sm[tid + g * DL] == top ? 1.f : fast_exp2((sm[tid + g * DL] - top) * a.sc);
-    l += x * sl[tid + g * DL];
-    o += x * so[tid + g * DL];
-  }
-  const int64_t bl = row / a.H, head = row - bl * a.H, b = bl / a.L, tok = bl - b * a.L;
-  // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
-  const int64_t own = a.own_len[b] > a.S ? a.S : a.own_len[b];
-  const float inv = a.P > 0 || own - a.L + tok + 1 > 0 ? 1.f / l : 0.f;
-  Tile::store4((T*)a.out + b * a.out_seq + tok * a.out_row + head * a.out_head + 4 * dl, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 }  // namespace pp
@@ -194,13 +117,7 @@ static int launch_prefix(void* stream, pp::PrefixK& a) {
   if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(Tile::kThreads), Tile::kSmem, stream, a);
   const int rc = pp_check_launch("pp_prefix_attention");
   if (rc != PP_OK) return rc;
-  constexpr int DL = Tile::kDB <= 1 ? 8 : Tile::kDB <= 2 ? 16 : Tile::kDB <= 4 ? 32 : 64;
-  int pg = 0;  // a part group gets up to 4 parts before there is another
-  while ((4 << pg) < a.parts && (2 << pg) * DL <= 256) ++pg;
-  const int64_t per = 256 / (DL << pg), blocks = ((int64_t)a.B * a.L * a.H + per - 1) / per;
-  if (blocks * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the join needs 2^32 threads or more");
-  PP_LAUNCH((prefix_join_kernel<Tile, DL>), dim3((unsigned)blocks), dim3(256), 0, stream, a, pg);
-  return pp_check_launch("pp_prefix_attention(join)");
+  return launch_join<Tile>(stream, a.parts, "pp_prefix_attention(join)");
 }
 
 template <typename T>
@@ -247,24 +164,27 @@ extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_p
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: tensors must be 16-byte aligned");
   if (p->B == 0 || p->L == 0) return PP_OK;  // no row to write
   PrefixK a;
-  a.q = p->q; a.kp = p->kp; a.vp = p->vp; a.ko = p->ko; a.vo = p->vo; a.out = p->out; a.own_len = (const int*)p->own_len;
+  a.q = p->q; a.kp = p->kp; a.vp = p->vp; a.ko = p->ko; a.vo = p->vo; a.own_len = (const int*)p->own_len;
   a.q_seq = p->q_seq; a.q_row = p->q_row; a.q_head = p->q_head;
   a.kp_row = p->kp_row; a.kp_head = p->kp_head; a.vp_row = p->vp_row; a.vp_head = p->vp_head;
   a.ko_seq = p->ko_seq; a.ko_row = p->ko_row; a.ko_head = p->ko_head;
   a.vo_seq = p->vo_seq; a.vo_row = p->vo_row; a.vo_head = p->vo_head;
-  a.out_seq = p->out_seq; a.out_row = p->out_row; a.out_head = p->out_head;
   a.P = p->P; a.S = p->S;
   a.B = (int)p->B; a.L = (int)p->L; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D;
   a.prefix_splits = p->P > 0 ? p->prefix_splits : 0;
   a.own_splits = p->S > 0 ? p->own_splits : 0;
-  a.parts = a.prefix_splits + a.own_splits;
   a.sc = p->scale * kLog2e;
   const int64_t rows = p->B * p->L * p->H;
   if (rows > ((int64_t)1 << 40) / 65536 || p->L * a.G > INT32_MAX / 2) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: too many rows");
   if (p->scratch_bytes < rows * (p->prefix_splits + p->own_splits) * (p->D + 4) * 4)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: scratch smaller than B * L * H * (prefix_splits + own_splits) * (D + 4) floats");
-  a.part_o = (float*)p->scratch;
-  a.part_ml = a.part_o + rows * a.parts * p->D;
+  PartsK& pt = a.parts;
+  pt.parts = a.prefix_splits + a.own_splits;
+  pt.o = (float*)p->scratch;
+  pt.ml = pt.o + rows * pt.parts * p->D;
+  pt.out = p->out; pt.out_seq = p->out_seq; pt.out_row = p->out_row; pt.out_head = p->out_head;
+  pt.lse = nullptr; pt.cu_q = nullptr; pt.ncu = 0;
+  pt.rows = rows; pt.L = a.L; pt.H = a.H; pt.D = a.D; pt.sc = a.sc; pt.scale = p->scale;
   if (p->dtype == PP_F32) return launch_prefix_d<float>(stream, a);
   if (p->dtype == PP_F16) return launch_prefix_d<half_t>(stream, a);
   return launch_prefix_d<bf16_t>(stream, a);

@@ -5,10 +5,12 @@
 // a work-group takes kRows of them, so short prompts fill its tiles with heads, and the keys of a group are staged once for all of its heads.
 // Tiles are numbered without knowing a length on the host: sequence s starts at tile floor(cu_q[s] G / kRows) + s, which leaves each at
 // least ceil(n G / kRows) numbers; a work-group finds its sequence by a 64-ary search over cu_q and returns if its number is spare.
-// Later tiles of a causal sequence see more keys and are launched first; the key / value head is the fastest index of the grid, so with 8 (or a
+// Later tiles of a causal sequence see more keys and are launched first.  (Ordering the tiles of all sequences by their keys was slower, 16 ragged
+// prompts of up to 2048 tokens: 130 -> 139 us -- neighbouring tiles of a sequence share its keys in the L2.)  The key / value head is the fastest index of the grid, so with 8 (or a
 // multiple or divisor of 8) of them a head's keys stay in the L2 of its XCDs.
-#include "tile_attention.h"
-#include "pp_host.h"
+// Few tiles with many keys leave most of the chip idle: with `splits` > 1 a tile's keys go to that many work-groups, whose parts a second
+// launch joins (attention_parts.h).
+#include "attention_parts.h"
 
 #include <math.h>
 
@@ -22,8 +24,9 @@ struct PromptK {
   float* lse;
   const int *cu_q, *cu_k;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, Tq, Tk;
-  int B, H, KH, G, D, causal, ntiles;
+  int B, H, KH, G, D, causal, ntiles, splits;
   float scale, sc;
+  PartsK parts;
 };
 
 __device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
@@ -35,11 +38,11 @@ template <typename Tile>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
   typedef typename Tile::type T;
   constexpr int kRows = Tile::kRows, RB = Tile::RB;
-  const int kh = (int)blockIdx.x % a.KH;
-  const int64_t tile = a.ntiles - 1 - (int)blockIdx.x / a.KH;
+  const int kh = (int)blockIdx.x % a.KH, split = (int)blockIdx.x / a.KH % a.splits;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
 
   // ---- the sequence that owns this tile: the last s with first_tile(s) <= tile
+  const int64_t tile = a.ntiles - 1 - (int)blockIdx.x / a.KH / a.splits;
   int s = 0;
   for (int n = a.B; n > 1;) {
     const int step = (n + 63) / 64, i = s + lane * step;
@@ -54,12 +57,20 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention
   const int64_t row0 = (tile - (q0 * a.G / kRows + s)) * kRows;
   if (row0 < 0 || row0 >= rows) return;
 
-  // ---- what the rows see
+  // ---- what the rows see of the keys [first, first + most)
+  int first = 0;
+  int64_t most = m;
   auto limit_of = [&](int64_t row) __attribute__((always_inline)) -> int {
-    const int64_t c = a.causal ? row / a.G + 1 + m - n : m;
-    return (int)(c < 0 ? 0 : c > m ? m : c);
+    const int64_t c = (a.causal ? row / a.G + 1 + m - n : m) - first;
+    return (int)(c < 0 ? 0 : c > most ? most : c);
   };
   const int64_t last = rows - 1, wrow = row0 + 32 * RB * wave;
+  if (a.splits > 1) {
+    const int all = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
+    const int per = ((all + a.splits - 1) / a.splits + 63) / 64 * 64;
+    first = split * per < all ? split * per : all;
+    most = all - first < per ? all - first : per;
+  }
   AttnLimits<RB> lim;
   lim.wave_min = wrow <= last ? limit_of(wrow) : 0;
   lim.wave_max = wrow <= last ? limit_of(wrow + 32 * RB - 1 < last ? wrow + 32 * RB - 1 : last) : 0;
@@ -75,14 +86,20 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention
     lim.row[rb] = live ? limit_of(row) : 0;
     t.load_q(rb, live ? (const T*)a.q + (q0 + row / a.G) * a.q_row + (kh * a.G + row % a.G) * a.q_head : nullptr, a.D);
   }
-  attend(t, st, (const T*)a.k + k0 * a.k_row + kh * a.k_head, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.k_row, a.v_row, lim, a.D, a.sc);
-  if (st.not_finite) add_not_finite(t, st, (const T*)a.v + k0 * a.v_row + kh * a.v_head, a.v_row, lim, a.D);
+  const T* k = (const T*)a.k + (k0 + first) * a.k_row + kh * a.k_head;
+  const T* v = (const T*)a.v + (k0 + first) * a.v_row + kh * a.v_head;
+  attend(t, st, k, v, a.k_row, a.v_row, lim, a.D, a.sc);
+  if (st.not_finite) add_not_finite(t, st, v, a.v_row, lim, a.D);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int64_t row = wrow + 32 * rb + q32;
     if (row > last) continue;
     const int64_t token = q0 + row / a.G;
     const int head = kh * a.G + (int)(row % a.G);
+    if (a.splits > 1) {
+      store_part(a.parts, t, st, rb, token * a.H + head, split, lim.row[rb] > 0);
+      continue;
+    }
     // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
     const float inv = lim.row[rb] > 0 ? 1.f / st.l[rb] : 0.f;
     T* dst = (T*)a.out + token * a.out_row + head * a.out_head;
@@ -104,11 +121,12 @@ template <typename Tile>
 static int launch_prompt(void* stream, pp::PromptK& a) {
   using namespace pp;
   const int64_t ntiles = a.Tq * a.G / Tile::kRows + a.B;
-  if (ntiles * a.KH * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
+  if (ntiles * a.KH * a.splits * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
   a.ntiles = (int)ntiles;
   PP_ALLOW_BIG_LDS((&prompt_attention_kernel<Tile>), Tile::kSmem);
-  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
-  return pp_check_launch("pp_prompt_attention");
+  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH * a.splits)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
+  const int rc = pp_check_launch("pp_prompt_attention");
+  return rc != PP_OK || a.splits == 1 ? rc : launch_join<Tile>(stream, a.parts, "pp_prompt_attention(join)");
 }
 
 template <typename T>
@@ -156,6 +174,10 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
     if (row >= 1 << 24) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: a key or value row stride must be below 2^24 elements");
   if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) % 16)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: tensors must be 16-byte aligned");
+  const int splits = p->splits ? p->splits : 1;
+  if (splits < 1 || splits > 64) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: splits must be in [0, 64]");
+  if (splits > 1 && (!p->scratch || (uintptr_t)p->scratch % 16 || p->scratch_bytes / (splits * (p->D + 4) * 4) < p->Tq * p->H))
+    return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: splits need a 16-byte aligned scratch of Tq * H * splits * (D + 4) floats");
   if (p->B == 0 || p->Tq == 0) return PP_OK;  // no row to write
   PromptK a;
   a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = (float*)p->lse;
@@ -165,6 +187,15 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
   a.Tq = p->Tq; a.Tk = p->Tk;
   a.B = (int)p->B; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D; a.causal = p->causal != 0;
   a.scale = p->scale; a.sc = p->scale * kLog2e;
+  a.splits = splits;
+  if (splits > 1) {
+    PartsK& pt = a.parts;
+    pt.rows = p->Tq * p->H; pt.L = (int)p->Tq; pt.H = a.H; pt.D = a.D; pt.parts = splits;
+    pt.o = (float*)p->scratch;
+    pt.ml = pt.o + pt.rows * splits * p->D;
+    pt.out = p->out; pt.out_seq = 0; pt.out_row = p->out_row; pt.out_head = p->out_head;
+    pt.lse = a.lse; pt.cu_q = a.cu_q; pt.ncu = a.B; pt.sc = a.sc; pt.scale = a.scale;
+  }
   if (p->dtype == PP_F32) return launch_prompt_d<float>(stream, a);
   if (p->dtype == PP_F16) return launch_prompt_d<half_t>(stream, a);
   return launch_prompt_d<bf16_t>(stream, a);

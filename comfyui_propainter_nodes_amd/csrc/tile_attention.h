@@ -299,7 +299,7 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
   static_assert(RB_ == 1 && NS_ == 1, "f32: one row block, 32 keys a step");
   static constexpr int NW = NW_, RB = 1, NS = 1, kThreads = 64 * NW, kBN = 32, kRows = 32 * NW;
   static constexpr bool kSteady = false;  // (the vector work is a twentieth of the matrix work: nothing to overlap by hand)
-  static constexpr int kWaves = DP > 128 ? 1 : 2;  // per SIMD
+  static constexpr int kWaves = DP > 128 || (DP > 96 && NW == 2) ? 1 : 2;  // per SIMD; LDS holds no more
   static constexpr int kP = DP + 4;
   static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 8;
   static constexpr int kSlot = kBN * kP, kFlag = 4 * kSlot * 4, kSmem = kFlag + 16;

@@ -1163,12 +1163,13 @@ def _writable(name: str, t: torch.Tensor) -> None:
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
-                     lse: torch.Tensor | None = None) -> torch.Tensor:
+                     lse: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over packed sequences: q, out [Tq,H,D], k, v [Tk,KH,D] (any strides, dense last dim; f16 / bf16 / fp32), H a multiple of
     KH; sequence s = query rows cu_q[s]:cu_q[s+1] and key rows cu_k[s]:cu_k[s+1] (i32 on the device; cu_k None: cu_q).  causal: query i of
     n sees key j of m if j <= i + m - n.  A query without a key gets 0; rows outside every sequence are left as they were.
     scale: 1/sqrt(D) by default.  lse: fp32 [Tq,H], ln of the softmax sums (-inf without a key).  out may be q; it must not overlap
-    k or v."""
+    k or v.  `scratch`: float32, prompt_attention_scratch() elements (0 for most calls); by default a tensor of this call's own, so that two
+    captured graphs or two streams never share one.  A caller that passes its own must not let two calls run on it at once."""
     cu_k = cu_q if cu_k is None else cu_k
     check_device(q, k, v, out, cu_q, cu_k, lse)
     qs, ks, vs, os_ = _heads_view("q", q, 3), _heads_view("k", k, 3), _heads_view("v", v, 3), _heads_view("out", out, 3)
@@ -1183,13 +1184,39 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
             raise ValueError(f"prompt_attention: {name} must be a dense int32 [sequences + 1] tensor")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tq, h) or not lse.is_contiguous()):
         raise ValueError(f"prompt_attention: lse must be a dense fp32 [{tq}, {h}] tensor")
+    splits = prompt_splits(cu_q.numel() - 1, tq, tk, h, kh)
+    at = need = 0
+    if splits > 1:
+        need = tq * h * splits * (d + 4)
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        else:
+            check_device(scratch)
+            if scratch.dtype != torch.float32 or scratch.numel() < need or not scratch.is_contiguous():
+                raise ValueError(f"prompt_attention: scratch must be a dense float32 tensor of at least {need} elements")
+        at = scratch.data_ptr()
     if tq > 0:
         qp = q.data_ptr()
         _lib.current().call_packed("pp_prompt_attention", stream_handle(out), _PROMPT.pack(
             code, int(causal), qp, *qs, k.data_ptr() if tk else qp, *ks, v.data_ptr() if tk else qp, *vs, out.data_ptr(), *os_,
             0 if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, tq, tk, h, kh, d,
-            d ** -0.5 if scale is None else scale))      # (tk = 0: every row is empty; an empty tensor has no address)
+            d ** -0.5 if scale is None else scale, splits, at, need * 4))      # (tk = 0: every row is empty; an empty tensor has no address)
     return out
+
+
+def prompt_splits(b: int, tq: int, tk: int, h: int, kh: int) -> int:
+    """Work-groups that share the keys of a tile in a prompt_attention call.  The chip holds 512 work-groups at once (two per CU); fewer tiles
+    than a third of that share their keys, as long as the average sequence leaves each work-group 256 of them.  (4096 causal tokens, 4 heads over
+    one key head of 128: 73 us alone, 47 in three parts; 4 x 1 token behind 8192 keys: 96 -> 23; 232 tiles of about 2000 keys: 31, in two parts 35.)"""
+    tiles = (tq * (h // kh) // 128 + b) * kh
+    splits = min(8, 512 // max(1, tiles), tk // max(1, b) // 256)
+    return splits if splits >= 3 else 1
+
+
+def prompt_attention_scratch(q: torch.Tensor, k: torch.Tensor, cu_q: torch.Tensor) -> int:
+    """float32 elements of scratch of a prompt_attention call on these tensors."""
+    splits = prompt_splits(cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1])
+    return 0 if splits == 1 else q.shape[0] * q.shape[1] * splits * (q.shape[2] + 4)
 
 
 def prefix_splits(b: int, new: int, p: int, s: int, h: int, kh: int) -> tuple[int, int]:

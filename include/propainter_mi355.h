@@ -567,6 +567,9 @@ typedef struct {
   const void* cu_k; /* i32 [B + 1] */
   int64_t B, Tq, Tk, H, KH, D;
   float scale; /* > 0, finite */
+  int32_t splits; /* work-groups that share the keys of a tile of rows (0 = 1): for few rows with many keys */
+  void* scratch;  /* splits > 1: caller-owned, 16-byte aligned, Tq * H * splits * (D + 4) floats */
+  int64_t scratch_bytes;
 } pp_prompt_attention_params;
 int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p);
 

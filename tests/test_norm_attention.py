@@ -303,6 +303,39 @@ def test_prompt_attention_offsets_out_of_range_stay_inside(emu_lib):
         assert bool(out.isfinite().all())
 
 
+@DT
+@pytest.mark.parametrize("lq,lk,causal", [([3, 1], [1100, 900], True), ([40], [800], False), ([800], [800], True), ([2, 0, 5], [3, 2400, 0], True)])
+def test_prompt_attention_keys_shared_by_work_groups(backend, dt, lq, lk, causal):
+    """Few rows with many keys: the keys of a tile go to several work-groups; parts without a key, rows without one, rows behind the last
+    sequence (tail of q / k / v beyond every offset)."""
+    assert ops.prompt_splits(len(lq), sum(lq) + 4, sum(lk) + 4, 2, 1) > 1
+    _check_prompt(backend, dt, 2, 1, 32, lq, lk, causal, tail=4)
+
+
+def test_prompt_attention_split_scratch(emu_lib):
+    q, k = torch.zeros(2, 2, 32), torch.zeros(1024, 1, 32)
+    cu_q, cu_k, out = torch.tensor([0, 2], dtype=torch.int32), torch.tensor([0, 1024], dtype=torch.int32), torch.empty(2, 2, 32)
+    need = ops.prompt_attention_scratch(q, k, cu_q)
+    assert need == 2 * 2 * 4 * 36
+    ops.prompt_attention(q, k, k, out, cu_q, cu_k, scratch=torch.empty(need))
+    with pytest.raises(ValueError, match="scratch"):
+        ops.prompt_attention(q, k, k, out, cu_q, cu_k, scratch=torch.empty(need - 1))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attention_more_tiles_than_fit_at_once(backend, causal):
+    """More tiles than the chip holds at once, several sequences, spare tile numbers between them: every row comes out once."""
+    lq, lk = [30, 0, 1, 17, 40, 8], [30, 5, 40, 9, 40, 0]
+    h = kh = 96
+    assert (sum(lq) // 128 + len(lq)) * kh > 512
+    _check_prompt(backend, F16, h, kh, 32, lq, lk, causal, tail=2)
+
+
+@gpu_only
+def test_prompt_attention_many_long_tiles(hip_lib):
+    _check_prompt(torch.device("cuda:0"), BF16, 64, 8, 64, [300, 900, 1, 512, 0, 77], [300, 1000, 700, 512, 3, 77], True)
+
+
 def test_prompt_attention_many_sequences(backend):
     """The search over the offsets takes more than one step beyond 64 sequences."""
     lens = [(7 * i) % 5 for i in range(150)]
