@@ -20,18 +20,19 @@ struct PartsK {
 };
 
 template <typename Tile>
-__device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const AttnState<Tile>& st, int rb, int64_t row, int part, bool any) {
+__device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const AttnState<Tile>& st, int rb, int64_t row, int part, bool any, int d0,
+                                           int DV) {  // channels d0 .. d0 + DV - 1
   const int64_t at = row * a.parts + part;
-  float* dst = a.o + at * a.D;
+  float* dst = a.o + at * a.D + d0;
 #pragma unroll
   for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * db + 8 * g + 4 * t.h;
       const f16v& o = st.o[rb][db];
-      if (d < a.D) *reinterpret_cast<f4*>(dst + d) = f4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
+      if (d < DV) *reinterpret_cast<f4*>(dst + d) = f4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
     }
-  if (t.h == 0) {
+  if (t.h == 0 && d0 == 0) {
     a.ml[2 * at] = st.m[rb];
     a.ml[2 * at + 1] = any ? st.l[rb] : -1.f;
   }
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const PartsK a, int
 
 template <typename Tile>
 int launch_join(void* stream, const PartsK& a, const char* who) {
-  constexpr int DL = Tile::kDB <= 1 ? 8 : Tile::kDB <= 2 ? 16 : Tile::kDB <= 4 ? 32 : 64;
+  constexpr int DP = Tile::kDB * 32 * Tile::kHalves, DL = DP <= 32 ? 8 : DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
   int pg = 0;  // a part group gets up to 4 parts before there is another
   while ((4 << pg) < a.parts && (2 << pg) * DL <= 256) ++pg;
   const int64_t per = 256 / (DL << pg), blocks = (a.rows + per - 1) / per;

@@ -30,8 +30,11 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
   typedef typename Tile::type T;
   constexpr int kRows = Tile::kRows, RB = Tile::RB;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
-  const bool shared = (int64_t)blockIdx.x < a.prefix_items;
-  int64_t id = shared ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - a.prefix_items;
+  const int d0 = (int)blockIdx.x % Tile::kHalves * Tile::kDV;  // the value channels from d0 on
+  const int DV = a.D - d0 < Tile::kDV ? a.D - d0 : Tile::kDV;
+  int64_t id = (int64_t)blockIdx.x / Tile::kHalves;
+  const bool shared = id < a.prefix_items;
+  if (!shared) id -= a.prefix_items;
   const int kh = (int)(id % a.KH);
   id /= a.KH;
   const int lg = a.L * a.G;
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
     n0 = a.P * part / a.prefix_splits;
     n1 = a.P * (part + 1) / a.prefix_splits;
     k = (const T*)a.kp + kh * a.kp_head;
-    v = (const T*)a.vp + kh * a.vp_head;
+    v = (const T*)a.vp + kh * a.vp_head + d0;
     k_row = a.kp_row;
     v_row = a.vp_row;
   } else {
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
     n0 = visible * sp / a.own_splits;
     n1 = visible * (sp + 1) / a.own_splits;
     k = (const T*)a.ko + seq * a.ko_seq + kh * a.ko_head;
-    v = (const T*)a.vo + seq * a.vo_seq + kh * a.vo_head;
+    v = (const T*)a.vo + seq * a.vo_seq + kh * a.vo_head + d0;
     k_row = a.ko_row;
     v_row = a.vo_row;
   }
@@ -90,15 +93,15 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
     const int in_seq = (int)(shared ? row % lg : row);
     t.load_q(rb, live ? (const T*)a.q + b * a.q_seq + (in_seq / a.G) * a.q_row + (kh * a.G + in_seq % a.G) * a.q_head : nullptr, a.D);
   }
-  attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, lim, a.D, a.sc);
-  if (st.not_finite) add_not_finite(t, st, v + n0 * v_row, v_row, lim, a.D);
+  attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, lim, a.D, DV, a.sc);
+  if (st.not_finite) add_not_finite(t, st, v + n0 * v_row, v_row, lim, DV);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int64_t row = wrow + 32 * rb + q32;
     if (row > last) continue;
     const int64_t b = shared ? row / lg : seq;
     const int in_seq = (int)(shared ? row % lg : row);
-    store_part(a.parts, t, st, rb, (b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G, part, lim.row[rb] > 0);
+    store_part(a.parts, t, st, rb, (b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G, part, lim.row[rb] > 0, d0, DV);
   }
 }
 
@@ -112,9 +115,9 @@ static int launch_prefix(void* stream, pp::PrefixK& a) {
   a.own_tiles = (a.L * a.G + Tile::kRows - 1) / Tile::kRows;
   a.prefix_items = (int64_t)a.prefix_splits * a.prefix_tiles * a.KH;
   const int64_t items = a.prefix_items + (int64_t)a.own_splits * a.B * a.own_tiles * a.KH;
-  if (items * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the launch needs 2^32 threads or more");
+  if (items * Tile::kHalves * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: the launch needs 2^32 threads or more");
   PP_ALLOW_BIG_LDS((&prefix_attention_kernel<Tile>), Tile::kSmem);
-  if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)items), dim3(Tile::kThreads), Tile::kSmem, stream, a);
+  if (items > 0) PP_LAUNCH((prefix_attention_kernel<Tile>), dim3((unsigned)(items * Tile::kHalves)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
   const int rc = pp_check_launch("pp_prefix_attention");
   if (rc != PP_OK) return rc;
   return launch_join<Tile>(stream, a.parts, "pp_prefix_attention(join)");

@@ -38,11 +38,13 @@ template <typename Tile>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
   typedef typename Tile::type T;
   constexpr int kRows = Tile::kRows, RB = Tile::RB;
-  const int kh = (int)blockIdx.x % a.KH, split = (int)blockIdx.x / a.KH % a.splits;
+  const int id = (int)blockIdx.x / Tile::kHalves, d0 = (int)blockIdx.x % Tile::kHalves * Tile::kDV;  // the value channels from d0 on
+  const int DV = a.D - d0 < Tile::kDV ? a.D - d0 : Tile::kDV;
+  const int kh = id % a.KH, split = id / a.KH % a.splits;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
 
   // ---- the sequence that owns this tile: the last s with first_tile(s) <= tile
-  const int64_t tile = a.ntiles - 1 - (int)blockIdx.x / a.KH / a.splits;
+  const int64_t tile = a.ntiles - 1 - id / a.KH / a.splits;
   int s = 0;
   for (int n = a.B; n > 1;) {
     const int step = (n + 63) / 64, i = s + lane * step;
@@ -87,9 +89,9 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention
     t.load_q(rb, live ? (const T*)a.q + (q0 + row / a.G) * a.q_row + (kh * a.G + row % a.G) * a.q_head : nullptr, a.D);
   }
   const T* k = (const T*)a.k + (k0 + first) * a.k_row + kh * a.k_head;
-  const T* v = (const T*)a.v + (k0 + first) * a.v_row + kh * a.v_head;
-  attend(t, st, k, v, a.k_row, a.v_row, lim, a.D, a.sc);
-  if (st.not_finite) add_not_finite(t, st, v, a.v_row, lim, a.D);
+  const T* v = (const T*)a.v + (k0 + first) * a.v_row + kh * a.v_head + d0;
+  attend(t, st, k, v, a.k_row, a.v_row, lim, a.D, DV, a.sc);
+  if (st.not_finite) add_not_finite(t, st, v, a.v_row, lim, DV);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int64_t row = wrow + 32 * rb + q32;
@@ -97,21 +99,21 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention
     const int64_t token = q0 + row / a.G;
     const int head = kh * a.G + (int)(row % a.G);
     if (a.splits > 1) {
-      store_part(a.parts, t, st, rb, token * a.H + head, split, lim.row[rb] > 0);
+      store_part(a.parts, t, st, rb, token * a.H + head, split, lim.row[rb] > 0, d0, DV);
       continue;
     }
     // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
     const float inv = lim.row[rb] > 0 ? 1.f / st.l[rb] : 0.f;
-    T* dst = (T*)a.out + token * a.out_row + head * a.out_head;
+    T* dst = (T*)a.out + token * a.out_row + head * a.out_head + d0;
 #pragma unroll
     for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = 32 * db + 8 * g + 4 * h;
         const f16v& o = st.o[rb][db];
-        if (d < a.D) Tile::store4(dst + d, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
+        if (d < DV) Tile::store4(dst + d, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
       }
-    if (a.lse && h == 0) a.lse[token * a.H + head] = lim.row[rb] > 0 ? st.m[rb] * a.scale + logf(st.l[rb]) : neg_inf();
+    if (a.lse && h == 0 && d0 == 0) a.lse[token * a.H + head] = lim.row[rb] > 0 ? st.m[rb] * a.scale + logf(st.l[rb]) : neg_inf();
   }
 }
 
@@ -121,10 +123,10 @@ template <typename Tile>
 static int launch_prompt(void* stream, pp::PromptK& a) {
   using namespace pp;
   const int64_t ntiles = a.Tq * a.G / Tile::kRows + a.B;
-  if (ntiles * a.KH * a.splits * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
+  if (ntiles * a.KH * a.splits * Tile::kHalves * 256 >= ((int64_t)1 << 32)) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: the launch needs 2^32 threads or more");
   a.ntiles = (int)ntiles;
   PP_ALLOW_BIG_LDS((&prompt_attention_kernel<Tile>), Tile::kSmem);
-  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH * a.splits)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
+  PP_LAUNCH((prompt_attention_kernel<Tile>), dim3((unsigned)(a.ntiles * a.KH * a.splits * Tile::kHalves)), dim3(Tile::kThreads), Tile::kSmem, stream, a);
   const int rc = pp_check_launch("pp_prompt_attention");
   return rc != PP_OK || a.splits == 1 ? rc : launch_join<Tile>(stream, a.parts, "pp_prompt_attention(join)");
 }
@@ -174,6 +176,8 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
     if (row >= 1 << 24) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: a key or value row stride must be below 2^24 elements");
   if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) % 16)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: tensors must be 16-byte aligned");
+  if (p->out == p->q && p->dtype == PP_F32 && p->D > 128)  // two work-groups read a row's query, either may be done first
+    return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: out cannot be q for fp32 heads of more than 128 channels");
   const int splits = p->splits ? p->splits : 1;
   if (splits < 1 || splits > 64) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: splits must be in [0, 64]");
   if (splits > 1 && (!p->scratch || (uintptr_t)p->scratch % 16 || p->scratch_bytes / (splits * (p->D + 4) * 4) < p->Tq * p->H))

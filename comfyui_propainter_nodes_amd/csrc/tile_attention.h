@@ -130,13 +130,14 @@ struct AttnTile {
   static constexpr int kWaves = RB > 1 || DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kPitch = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
   static constexpr int kPieces = DP / 8, kPer = 8, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 16;
+  static constexpr int kHalves = 1, kDV = DP, kPiecesV = kPieces, kAllV = kAll, kStageV = kStage;
   static constexpr int kSlot = kBN * kPitch, kFlag = 4 * kSlot, kSmem = kFlag + 16;
   struct P {
     h8 f[2];
   };
 
   h8 q[RB][kQF];
-  u4 ks[kStage], vs[kStage];  // blocks on their way
+  u4 ks[kStage], vs[kStageV];  // blocks on their way
   unsigned char* smem;
   int q32, h;
 
@@ -301,14 +302,18 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
   static constexpr bool kSteady = false;  // (the vector work is a twentieth of the matrix work: nothing to overlap by hand)
   static constexpr int kWaves = DP > 128 || (DP > 96 && NW == 2) ? 1 : 2;  // per SIMD; LDS holds no more
   static constexpr int kP = DP + 4;
-  static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 8;
-  static constexpr int kSlot = kBN * kP, kFlag = 4 * kSlot * 4, kSmem = kFlag + 16;
+  // Queries of 256 channels and the sums of 256 do not fit the registers together (they spilled: 30 TF/s): two work-groups take half of the
+  // value channels each and both compute the scores, 3/2 of the work at four times the rate.
+  static constexpr int kHalves = DP > 128 ? 2 : 1, kDV = DP / kHalves;
+  static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = kDV / 32, kQF = DP / 8;
+  static constexpr int kPiecesV = kDV / 4, kAllV = kBN * kPiecesV, kStageV = (kAllV + kThreads - 1) / kThreads;
+  static constexpr int kPV = kDV + 4, kSlot = kBN * kP, kSlotV = kBN * kPV, kFlag = (2 * kSlot + 2 * kSlotV) * 4, kSmem = kFlag + 16;
   struct P {
     float f[16];
   };
 
   f4 q[1][kQF];
-  u4 ks[kStage], vs[kStage];
+  u4 ks[kStage], vs[kStageV];
   float* smem;
   int q32, h;
 
@@ -329,7 +334,7 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
     *reinterpret_cast<u4*>(smem + slot * kSlot + row * kP + 4 * piece) = ks[i];
   }
   __device__ __forceinline__ void store_v(int slot, int i, int row, int piece) const {
-    *reinterpret_cast<u4*>(smem + (2 + slot) * kSlot + row * kP + 4 * piece) = vs[i];
+    *reinterpret_cast<u4*>(smem + 2 * kSlot + slot * kSlotV + row * kPV + 4 * piece) = vs[i];
   }
   // channels are taken in the order (8c + 4h + j): any order serves a dot product as long as both operands share it
   __device__ __forceinline__ void qk(int slot, f16v (*s)[1]) const {
@@ -348,7 +353,7 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
     for (int r = 0; r < 16; ++r) f.f[r] = p[r];
     return f;
   }
-  __device__ __forceinline__ float v_val(int slot, int r, int db) const { return smem[(2 + slot) * kSlot + score_key(r, h) * kP + 32 * db + q32]; }
+  __device__ __forceinline__ float v_val(int slot, int r, int db) const { return smem[2 * kSlot + slot * kSlotV + score_key(r, h) * kPV + 32 * db + q32]; }
   // keys: wave-uniform; groups of 8 keys behind the last one that any row sees are left out
   __device__ __forceinline__ void pv(int slot, const P (*p)[1], f16v (*o)[kDB], int keys) const {
 #pragma unroll
@@ -392,10 +397,10 @@ struct AttnLimits {
   int row[RB], wave_min, wave_max, group_min, nkeys;
 };
 
-// k, v: the first key.  sc = scale * log2(e) > 0.
+// k, v: the first key; D, DV: their channels (of v: those from the pointer on that this work-group sums).  sc = scale * log2(e) > 0.
 template <typename Tile>
 __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typename Tile::type* k, const typename Tile::type* v,
-                                       int64_t k_row, int64_t v_row, const AttnLimits<Tile::RB>& lim, int D, float sc) {
+                                       int64_t k_row, int64_t v_row, const AttnLimits<Tile::RB>& lim, int D, int DV, float sc) {
   typedef typename Tile::type T;
   typedef typename Tile::P P;
   constexpr int RB = Tile::RB, NS = Tile::NS, BN = Tile::kBN;
@@ -413,30 +418,33 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   if (nsteps <= 0) return;
 
   // ---- staging: thread -> 16-byte pieces of a block; a piece past the head dim has an offset that no block reaches
-  unsigned koff[Tile::kStage], voff[Tile::kStage];
+  unsigned koff[Tile::kStage], voff[Tile::kStageV];
 #pragma unroll
   for (int i = 0; i < Tile::kStage; ++i) {
     const int at = (int)threadIdx.x + Tile::kThreads * i, row = at / Tile::kPieces, piece = at - row * Tile::kPieces;
-    const bool in = piece * Tile::kPer < D && row < BN;
-    koff[i] = in ? (unsigned)(row * k_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
-    voff[i] = in ? (unsigned)(row * v_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
+    koff[i] = piece * Tile::kPer < D && row < BN ? (unsigned)(row * k_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
+  }
+#pragma unroll
+  for (int i = 0; i < Tile::kStageV; ++i) {
+    const int at = (int)threadIdx.x + Tile::kThreads * i, row = at / Tile::kPiecesV, piece = at - row * Tile::kPiecesV;
+    voff[i] = piece * Tile::kPer < DV && row < BN ? (unsigned)(row * v_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
   }
   const int mixed_from = lim.group_min;  // from this key on some rows see what others do not
   volatile int* const flag = reinterpret_cast<volatile int*>(reinterpret_cast<unsigned char*>(t.smem) + Tile::kFlag);
   if (threadIdx.x == 0) *flag = 0;
-  auto block_of = [&](const T* base, int64_t stride, int i) __attribute__((always_inline)) -> Rows16 {
+  auto block_of = [&](const T* base, int64_t stride, int i, int channels) __attribute__((always_inline)) -> Rows16 {
     const int left = lim.nkeys - i * BN < BN ? lim.nkeys - i * BN : BN;
-    return rows16(base + (int64_t)i * BN * stride, left > 0 ? (unsigned)((left - 1) * stride + D) * (unsigned)sizeof(T) : 0u);
+    return rows16(base + (int64_t)i * BN * stride, left > 0 ? (unsigned)((left - 1) * stride + channels) * (unsigned)sizeof(T) : 0u);
   };
   auto load_k = [&](u4* dst, int i) __attribute__((always_inline)) {
-    const Rows16 block = block_of(k, k_row, i);
+    const Rows16 block = block_of(k, k_row, i, D);
 #pragma unroll
     for (int j = 0; j < Tile::kStage; ++j) dst[j] = load_row16(block, koff[j]);
   };
   auto load_v = [&](int i) __attribute__((always_inline)) {
-    const Rows16 block = block_of(v, v_row, i);
+    const Rows16 block = block_of(v, v_row, i, DV);
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) t.vs[j] = load_row16(block, voff[j]);
+    for (int j = 0; j < Tile::kStageV; ++j) t.vs[j] = load_row16(block, voff[j]);
   };
   auto store_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -447,9 +455,9 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   };
   auto store_v = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < Tile::kStage; ++j) {
-      const int at = (int)threadIdx.x + Tile::kThreads * j, row = at / Tile::kPieces;
-      if (Tile::kAll % Tile::kThreads == 0 || at < Tile::kAll) t.store_v(slot, j, row, at - row * Tile::kPieces);
+    for (int j = 0; j < Tile::kStageV; ++j) {
+      const int at = (int)threadIdx.x + Tile::kThreads * j, row = at / Tile::kPiecesV;
+      if (Tile::kAllV % Tile::kThreads == 0 || at < Tile::kAllV) t.store_v(slot, j, row, at - row * Tile::kPiecesV);
     }
   };
 
@@ -544,7 +552,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     const int s0 = i & 1, s1 = 1 - s0;
     if (mixed_from < lim.nkeys && (i + 1) * BN > mixed_from) {
 #pragma unroll
-      for (int j = 0; j < Tile::kStage; ++j)
+      for (int j = 0; j < Tile::kStageV; ++j)
         if (Tile::scrub(t.vs[j])) *flag = 1;
     }
     stage(i, s0);
@@ -606,7 +614,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
 // with a key that not every row of the work-group sees.
 template <typename Tile>
 __device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& st, const typename Tile::type* v, int64_t v_row,
-                                               const AttnLimits<Tile::RB>& lim, int D) {
+                                               const AttnLimits<Tile::RB>& lim, int DV) {
 #pragma unroll 1
   for (int key = lim.group_min / Tile::kBN * Tile::kBN; key < lim.nkeys; ++key) {
     const typename Tile::type* row = v + key * v_row;
@@ -615,7 +623,7 @@ __device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& s
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int d = 32 * db + score_key(r, t.h);
-        const float x = d < D ? to_f32(row[d]) : 0.f;
+        const float x = d < DV ? to_f32(row[d]) : 0.f;
         if ((__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u) {
 #pragma unroll
           for (int rb = 0; rb < Tile::RB; ++rb)

@@ -548,6 +548,7 @@ int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p);
  * The offsets live on the device: values outside [0, Tq] / [0, Tk] are clamped, a sequence of negative length is empty.
  * Strides in elements, those of key and value rows below 2^24; the last dim is dense; every row start is 16-byte aligned;
  * D % 8 == 0 (% 4 for PP_F32), D <= 256.
+ * out may be q (same strides; not for PP_F32 with D > 128), and overlaps nothing else.
  * PP_F16 / PP_BF16: MFMA operands in the storage type (the probabilities are rounded to it once, as operands of the second
  * product), fp32 scores, sums and accumulators.  PP_F32: everything fp32 (f32 MFMA).
  * ---------------------------------------------------------------------------------- */

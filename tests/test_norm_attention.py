@@ -312,6 +312,25 @@ def test_prompt_attention_keys_shared_by_work_groups(backend, dt, lq, lk, causal
     _check_prompt(backend, dt, 2, 1, 32, lq, lk, causal, tail=4)
 
 
+def test_attention_in_place(backend):
+    g = torch.Generator().manual_seed(71)
+    q, k, v = (torch.randn(70, n, 64, generator=g).to(F16).to(backend) for n in (4, 2, 2))
+    cu, want = _cu([30, 40], backend), torch.empty_like(q)
+    ops.prompt_attention(q, k, v, want, cu)
+    x = q.clone()
+    ops.prompt_attention(x, k, v, x, cu)
+    assert torch.equal(x, want)
+    n = torch.tensor([3, 0], dtype=torch.int32, device=backend)
+    own = torch.randn(2, 3, 2, 64, generator=g).to(F16).to(backend)
+    ops.prefix_attention(q[:2], k, v, own, own, n, want[:2])
+    x = q[:2].clone()
+    ops.prefix_attention(x, k, v, own, own, n, x)
+    assert torch.equal(x, want[:2])
+    wide = torch.zeros(70, 2, 160, device=backend)
+    with pytest.raises(RuntimeError, match="cannot be q"):
+        ops.prompt_attention(wide, wide, wide, wide, cu)
+
+
 def test_prompt_attention_split_scratch(emu_lib):
     q, k = torch.zeros(2, 2, 32), torch.zeros(1024, 1, 32)
     cu_q, cu_k, out = torch.tensor([0, 2], dtype=torch.int32), torch.tensor([0, 1024], dtype=torch.int32), torch.empty(2, 2, 32)
