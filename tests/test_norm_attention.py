@@ -145,6 +145,10 @@ def test_groupnorm_refusals(emu_lib):
         ops.groupnorm(x, y, 4, eps=-1.0)
     with pytest.raises(KeyError):       # the convolutions do not take the new activation
         ops.conv2d(ops.make_conv_spec(torch.zeros(32, 32, 1, 1), None, F32), [torch.zeros(1, 4, 4, 32)], torch.empty(1, 4, 4, 32), act="silu")
+    P = ops._conv2d_params(ops.make_conv_spec(torch.zeros(32, 32, 1, 1), None, F32), [torch.zeros(1, 4, 4, 32)], torch.empty(1, 4, 4, 32))
+    P.act = lib.CONSTS["PP_ACT_SILU"]
+    with pytest.raises(RuntimeError, match="PP_ACT_SILU"):
+        lib.current().call("pp_conv2d", 0, P)
     e = torch.empty(0, 4, 4, 16)
     assert ops.groupnorm(e, torch.empty_like(e), 4).shape == e.shape
 
@@ -345,7 +349,7 @@ def test_prompt_attention_split_scratch(emu_lib):
 def test_prompt_attention_more_tiles_than_fit_at_once(backend, causal):
     """More tiles than the chip holds at once, several sequences, spare tile numbers between them: every row comes out once."""
     lq, lk = [30, 0, 1, 17, 40, 8], [30, 5, 40, 9, 40, 0]
-    h = kh = 96
+    h = kh = 100
     assert (sum(lq) // 128 + len(lq)) * kh > 512
     _check_prompt(backend, F16, h, kh, 32, lq, lk, causal, tail=2)
 
