@@ -392,8 +392,8 @@ extern "C" int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p) {
   using namespace pp;
   if (!p || !p->x || !p->y || !p->partials) return pp_fail(PP_ERR_BAD_ARG, "pp_groupnorm: null argument");
   if (p->dtype != PP_F32 && p->dtype != PP_F16 && p->dtype != PP_BF16) return pp_fail(PP_ERR_UNSUPPORTED, "pp_groupnorm: dtype");
-  if (p->N < 0 || p->HW < 0 || p->C < 1 || p->C > 65536 || p->groups < 1 || p->C % p->groups)
-    return pp_fail(PP_ERR_BAD_ARG, "pp_groupnorm: C must be in [1, 65536] and a multiple of groups");
+  if (p->N < 0 || p->HW < 0 || p->HW > (int64_t)1 << 40 || p->C < 1 || p->C > 65536 || p->groups < 1 || p->C % p->groups)
+    return pp_fail(PP_ERR_BAD_ARG, "pp_groupnorm: C must be in [1, 65536] and a multiple of groups, HW at most 2^40");
   if (p->act < PP_ACT_NONE || p->act > PP_ACT_SILU) return pp_fail(PP_ERR_BAD_ARG, "pp_groupnorm: act");
   if (p->x_ldc < p->C || p->y_ldc < p->C || (p->skip && p->skip_ldc < p->C))
     return pp_fail(PP_ERR_BAD_ARG, "pp_groupnorm: channel pitch smaller than C");

@@ -180,8 +180,10 @@ extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_p
   a.prefix_splits = p->P > 0 ? p->prefix_splits : 0;
   a.own_splits = p->S > 0 ? p->own_splits : 0;
   a.sc = p->scale * kLog2e;
+  // (the products below stay inside 64 bits: B L and H are at most 2^24 and 2^20)
+  if (p->B * p->L > (1 << 24) || p->B * p->L * p->H > (1 << 24))
+    return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: more than 2^24 rows (B * L * H)");
   const int64_t rows = p->B * p->L * p->H;
-  if (rows > ((int64_t)1 << 40) / 65536 || p->L * a.G > INT32_MAX / 2) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: too many rows");
   if (p->scratch_bytes < rows * (p->prefix_splits + p->own_splits) * (p->D + 4) * 4)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: scratch smaller than B * L * H * (prefix_splits + own_splits) * (D + 4) floats");
   PartsK& pt = a.parts;

@@ -167,6 +167,8 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
   if (p->D < 1 || p->D > 256 || p->D % e) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: D must be a multiple of 8 (fp32: 4) up to 256");
   if (p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->B > INT32_MAX / 2 || p->Tq > INT32_MAX || p->Tk > INT32_MAX)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: B, Tq, Tk must be in [0, 2^31)");
+  if (p->Tq * p->H > (int64_t)1 << 40 || p->B * p->KH > (int64_t)1 << 32)  // (what is computed from them stays inside 64 bits)
+    return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: Tq * H or B * KH too large");
   if (!(p->scale > 0.f) || !(p->scale * kLog2e < INFINITY)) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: scale must be positive and finite");
   const int64_t strides[8] = {p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head, p->out_row, p->out_head};
   for (int i = 0; i < 8; ++i)

@@ -477,6 +477,31 @@ def test_prefix_attention_refusals(emu_lib):
         lib.current().call("pp_prefix_attention", 0, P)
 
 
+def test_sizes_that_no_launch_holds(emu_lib):
+    """Sizes whose products leave 64 bits are refused before anything is computed from them."""
+    one = torch.zeros(64)
+    at = one.data_ptr()
+    P = lib.STRUCTS["pp_prefix_attention_params"]()
+    P.q = P.kp = P.vp = P.ko = P.vo = P.own_len = P.out = P.scratch = at
+    P.prefix_splits = P.own_splits = 1
+    P.scale, P.B, P.L, P.H, P.KH, P.D, P.P, P.S = 1.0, 1 << 24, 1 << 20, 1 << 20, 1 << 20, 8, 1, 1
+    with pytest.raises(RuntimeError, match="2\\^24 rows"):
+        emu_lib.call("pp_prefix_attention", 0, P)
+    P = lib.STRUCTS["pp_prompt_attention_params"]()
+    P.q = P.k = P.v = P.out = P.cu_q = P.cu_k = at
+    P.scale, P.B, P.Tq, P.Tk, P.H, P.KH, P.D = 1.0, 1 << 29, 1 << 30, 1, 1 << 20, 1 << 20, 8
+    with pytest.raises(RuntimeError, match="too large"):
+        emu_lib.call("pp_prompt_attention", 0, P)
+    P.B, P.Tq, P.H, P.KH = 1, 1 << 30, 64, 64
+    with pytest.raises(RuntimeError, match="2\\^32 threads"):
+        emu_lib.call("pp_prompt_attention", 0, P)
+    P = lib.STRUCTS["pp_groupnorm_params"]()
+    P.x = P.y = P.partials = at
+    P.N, P.HW, P.C, P.groups, P.x_ldc, P.y_ldc, P.nchunks = 1, 1 << 50, 8, 1, 8, 8, 1
+    with pytest.raises(RuntimeError, match="HW"):
+        emu_lib.call("pp_groupnorm", 0, P)
+
+
 # --------------------------------------------------------------------------------------------
 # together
 # --------------------------------------------------------------------------------------------
