@@ -6,7 +6,7 @@
 // cut into pieces so that few rows still fill the chip; the own keys of a sequence (its L G rows) are work-groups of the same launch.  Every piece
 // leaves (maximum, sum, sum of weighted values) in fp32; a second launch joins them in piece order.
 //
-// 128 tokens behind 32768 keys, 64 / 8 heads of 128, f16: 176-190 us (138 GF; the prefix part at the rate of a long prompt, one wave of four in
+// 128 tokens behind 32768 keys, 64 / 8 heads of 128, f16: 176-200 us (138 GF; the prefix part at the rate of a long prompt, one wave of four in
 // the own part); 32 tokens behind 8192 keys, 32 / 8 heads, bf16: 25 us, 20 + 5 for the join -- 8-10 steps per work-group, each waits for memory.
 #include "attention_parts.h"
 

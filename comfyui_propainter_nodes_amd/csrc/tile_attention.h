@@ -14,7 +14,7 @@
 // up rescaled and the block taken again.  No maximum is computed otherwise.  A probability is at most kMost, inside f16 and as exact as any other
 // relative to its own size, and the sum of a row is at least 1, the weight of the key that m came from.
 //
-// Bound by the matrix pipes: one causal prompt of 8192 tokens, 32 query heads over 8 key heads of 128, f16: 533-553 us by card = 1.0 PF/s, MFMA busy
+// Bound by the matrix pipes: one causal prompt of 8192 tokens, 32 query heads over 8 key heads of 128, f16: 533-590 us by card, 0.93-1.03 PF/s, MFMA busy
 // 52 % of the cycles at the 1.87 GHz that the card holds under it, LDS 39 %, no bank conflict; 843 TF/s at 64 channels, 860 at 256, f32 136 TF/s
 // (full f32 MFMA rate 157).  RB is 1 everywhere: 64 rows a wave halve the LDS reads, but leave one wave per SIMD and cost register moves (935 us).
 // With a maximum per block and per-lane addresses the same call took 703 us, with the MFMAs left to the compiler's order 634.

@@ -93,6 +93,8 @@ def _groupnorm_case(dev, dt, shape, groups, act, skip=False, affine=True, pitch=
     ((1, 3, 3, 2304), 2, "none", dict()),                      # more columns than a work-group holds at once
     ((1, 2, 3, 515), 5, "none", dict()),
     ((4, 40, 33, 64), 8, "relu", dict()),                      # several pieces per image
+    ((1, 32, 32, 16), 2, "silu", dict(skip=True)),             # 1024 vectors a group in 16-bit storage: the largest held in registers
+    ((1, 32, 33, 16), 2, "silu", dict(skip=True)),             # ... and the next, in two launches
 ])
 def test_groupnorm(backend, dt, shape, groups, act, kw):
     _groupnorm_case(backend, dt, shape, groups, act, **kw)
