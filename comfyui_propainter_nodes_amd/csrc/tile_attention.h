@@ -21,8 +21,8 @@
 //
 // Rows that see different numbers of keys: `limit` is the row's own count, scores at or past it become -inf before the softmax.  Their
 // probability is 0, but 0 x V is NaN for a V that is not finite.  Keys past the last one that any row of the work-group sees are staged as
-// zeros; in blocks that only some rows see, V values that are not finite are staged as zeros too, and if there were any, add_not_finite()
-// goes over those blocks once more at the end and adds them to the rows that do see them.
+// zeros, or as they are where rows overlap; in blocks that only some rows see, and in such a last block, V values that are not finite are staged
+// as zeros too, and if there were any, add_not_finite() goes over those blocks once more at the end and adds them to the rows that do see them.
 #pragma once
 #include "attn_device.h"
 #include "bf16_device.h"
@@ -402,6 +402,15 @@ struct AttnLimits {
   int row[RB], wave_min, wave_max, group_min, nkeys;
 };
 
+// The key from whose block on V is staged without values that are not finite: the first one that not every row sees -- or, where rows
+// lie closer together than their channels (a single row, an expanded or overlapping view), the first of a last block with rows left: such a row
+// starts before the block's last byte, so it is not read as zeros, and its weight of 0 does not make an infinity go away.
+template <typename Tile>
+__device__ __forceinline__ int mixed_key(const AttnLimits<Tile::RB>& lim, int64_t v_row, int DV) {
+  const int whole = lim.nkeys / Tile::kBN * Tile::kBN;
+  return v_row < DV && whole < lim.group_min ? whole : lim.group_min;
+}
+
 // k, v: the first key; D, DV: their channels (of v: those from the pointer on that this work-group sums).  sc = scale * log2(e) > 0.
 template <typename Tile>
 __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typename Tile::type* k, const typename Tile::type* v,
@@ -434,7 +443,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     const int at = (int)threadIdx.x + Tile::kThreads * i, row = at / Tile::kPiecesV, piece = at - row * Tile::kPiecesV;
     voff[i] = piece * Tile::kPer < DV && row < BN ? (unsigned)(row * v_row + piece * Tile::kPer) * sizeof(T) : ~0u << 5;
   }
-  const int mixed_from = lim.group_min;  // from this key on some rows see what others do not
+  const int mixed_from = mixed_key<Tile>(lim, v_row, DV);
   volatile int* const flag = reinterpret_cast<volatile int*>(reinterpret_cast<unsigned char*>(t.smem) + Tile::kFlag);
   if (threadIdx.x == 0) *flag = 0;
   auto block_of = [&](const T* base, int64_t stride, int i, int channels) __attribute__((always_inline)) -> Rows16 {
@@ -615,13 +624,13 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   st.not_finite = *flag != 0;
 }
 
-// Adds to o (weighted sums, normalised or not) what attend() left out: infinities and NaN of the keys that a row sees, from the first block
-// with a key that not every row of the work-group sees.
+// Adds to o (weighted sums, normalised or not) what attend() left out: infinities and NaN of the keys that a row sees, from the block of
+// mixed_key() on.
 template <typename Tile>
 __device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& st, const typename Tile::type* v, int64_t v_row,
                                                const AttnLimits<Tile::RB>& lim, int DV) {
 #pragma unroll 1
-  for (int key = lim.group_min / Tile::kBN * Tile::kBN; key < lim.nkeys; ++key) {
+  for (int key = mixed_key<Tile>(lim, v_row, DV) / Tile::kBN * Tile::kBN; key < lim.nkeys; ++key) {
     const typename Tile::type* row = v + key * v_row;
 #pragma unroll
     for (int db = 0; db < Tile::kDB; ++db)
