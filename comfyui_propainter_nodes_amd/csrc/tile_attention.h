@@ -11,8 +11,13 @@
 // before they are stored, one barrier a step.
 // The maximum m that the probabilities 2^(s sc - m sc) refer to is a true one, but not the newest: a block is taken against the m it
 // finds, and only if a lane's sum over the block comes out above kMost (any probability would be then, or NaN) is m moved, what was summed
-// up rescaled and the block taken again.  No maximum is computed otherwise.  A probability is at most kMost, inside f16 and as exact as any other
-// relative to its own size, and the sum of a row is at least 1, the weight of the key that m came from.
+// up rescaled and the block taken again.  Otherwise a maximum is only computed where a lane has no m to go by: rows that see no key yet (rows behind
+// the last one of a tile among them, in every block that masks them) and the far scores below.
+// A probability is at most kMost, inside f16 and as exact as any other relative to its own size, and the sum of a row is 1 or more, the weight
+// of the key that m came from.  That rests on 2^((s - m) sc), where the difference is exact near m: m sc rounded to f32 is half a unit in
+// its last place off, which nothing cancels -- 2^-13 of a power of two below kFar, less than a 16-bit probability's own rounding, and whole powers
+// of two from 2^24 on.  So 16-bit blocks are weighed by one fma with the rounded -m sc while |m sc| < kFar, and every block by the difference
+// beyond it; f32 storage and the blocks that move m always take the difference.
 //
 // Bound by the matrix pipes: one causal prompt of 8192 tokens, 32 query heads over 8 key heads of 128, f16: 533-590 us by card, 0.93-1.03 PF/s, MFMA busy
 // 52 % of the cycles at the 1.87 GHz that the card holds under it, LDS 39 %, no bank conflict; 843 TF/s at 64 channels, 860 at 256, f32 136 TF/s
@@ -32,6 +37,7 @@
 namespace pp {
 
 constexpr float kMost = 4096.f;
+constexpr float kFar = 4096.f;  // |m sc| from which a block is not weighed by 2^(s sc - m sc)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 #ifdef PP_EMU
@@ -481,7 +487,9 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
   // that nothing is copied.
   Scores s, s2;
   Probs p, p2;
-  float nm[RB], bs[RB];  // -m sc (NaN before the first visible key: whatever a block holds, it is taken again); sums over the block
+  // -m sc (NaN before the first visible key and from kFar on: whatever a block holds, it is taken again by its differences from the
+  // maximum); sums over the block
+  float nm[RB], bs[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) nm[rb] = __builtin_nanf("");
   auto softmax = [&](const Scores& x, Probs& y) __attribute__((always_inline)) -> bool {  // x -> y, bs; did a sum come out too large?
@@ -494,7 +502,8 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+          if constexpr (Tile::kSteady) e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+          else e[r] = fast_exp2((x[rb][sub][r] - st.m[rb]) * sc);  // (no maximum yet: infinite or NaN, taken again)
           bs[rb] += e[r];
         }
         y[rb][sub] = Tile::pack_p(e);
@@ -515,10 +524,10 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
         for (int r = 0; r < 16; ++r) top = fmaxf(top, x[rb][sub][r]);
       top = fmaxf(st.m[rb], pair32_max(top));
       const float alpha = top == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - top) * sc);
-      const float use = top == neg_inf() ? 0.f : -top * sc;
+      const float base = top == neg_inf() ? 0.f : top;
       st.m[rb] = top;
       st.l[rb] *= alpha;
-      nm[rb] = top == neg_inf() ? __builtin_nanf("") : use;
+      nm[rb] = fabsf(top * sc) < kFar ? -top * sc : __builtin_nanf("");
 #pragma unroll
       for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
@@ -529,7 +538,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
         float e[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, use));
+          e[r] = fast_exp2((x[rb][sub][r] - base) * sc);
           bs[rb] += e[r];
         }
         y[rb][sub] = Tile::pack_p(e);

@@ -76,3 +76,98 @@ def test_expanded_and_overlapping_rows(backend, dt, n):
         none = kk[:0].expand(0, 1, d)
         ops.prefix_attention(dq, kk, vv, none.expand(5, 0, 1, d), none.expand(5, 0, 1, d), _i32([0] * 5, backend), out)
         _expect(out, q, kk.cpu(), vv.cpu(), _seen(5, n, False), (name, "prefix"))
+
+
+# --------------------------------------------------------------------------------------------
+# finite scores far from zero
+# --------------------------------------------------------------------------------------------
+def _far_case(dt, sign, e, step, n, m, d, g):
+    """Queries and keys whose scores (scale 1) are sign * 32761 * 2^e + step * c_j, c_j whole numbers in [-24, 0], exactly: (181 * 2^x) times
+    (181 * 2^y) and a product with a multiple of `step`, all inside every storage type, whose sum f32 holds.  Returns q [n,2,d], k [m,1,d], the
+    scores."""
+    c = -torch.randint(0, 25, (m,), generator=g)
+    top, fine = sign * 32761 * 2.0 ** e, 2.0 ** (round(math.log2(step)) // 2)
+    q, k = torch.zeros(n, 2, d), torch.zeros(m, 1, d)
+    q[..., 0], k[..., 0] = 181 * 2.0 ** (e // 2), sign * 181 * 2.0 ** (e - e // 2)
+    q[..., 1], k[:, 0, 1] = fine, step / fine * c
+    scores = top + step * c.double()
+    for t in (q, k):
+        assert torch.equal(t.to(dt).float(), t)
+    assert torch.equal((q[0, 0] * k[:, 0]).sum(-1).double(), scores)
+    return q.to(dt), k.to(dt), scores
+
+
+def _far_expect(got, scores, seen, v, dt, what):
+    """The scores are exact, so are their distances from the maximum; a distance times scale log2(e) is rounded twice, and a weight
+    whose distance passes 256 is below every other's rounding: 256 * 1.45 * 2^-23 and the exponential's own error stay below 2^-13.  16-bit storage: a
+    block may be weighed against a rounded maximum below 2^12, at most 2^-13 of a power of two off.  Twice that, and the usual rest."""
+    n, h, d = got.shape
+    o, amp = torch.zeros(n, h, d, dtype=torch.float64), torch.zeros(n, h, d, dtype=torch.float64)
+    for i in range(n):
+        s = scores[seen[i]]
+        if s.numel():
+            w = torch.softmax(s, 0)
+            vv = v.double().cpu()[seen[i], 0]
+            o[i], amp[i] = w @ vv, w @ vv.abs()
+    tol = _attn_tol(dt, o, amp, scores.numel(), 0, 0.0, _vmax(v)) + 2.0 ** -12 * amp
+    _within(got, o, tol, what)
+
+
+@DT
+@pytest.mark.parametrize("sign,e,step", [(1, -5, 0.25), (1, -2, 0.25), (1, 5, 0.25), (-1, 5, 1.0), (1, 10, 4.0), (-1, 15, 256.0), (1, 15, 64.0),
+                                         (1, 25, 2.0 ** 16)])
+def test_scores_far_from_zero(backend, dt, sign, e, step):
+    """Scores of 10^3 to 10^12: a product with scale * log2(e) rounds them by up to thousands of units, their distances from the maximum are
+    exact."""
+    if dt == F16 and e > 16:
+        pytest.skip("no such product of two f16 values")
+    top = (sign, e)
+    g = torch.Generator().manual_seed(3)
+    n, m, d = 40, 330, 32
+    q, k, scores = _far_case(dt, sign, e, step, n, m, d, g)
+    v = torch.randn(m, 1, d, generator=g).to(dt)
+    dq, dk, dv = q.to(backend), k.to(backend), v.to(backend)
+    for causal in (False, True):
+        out, lse = torch.empty_like(dq), torch.empty(n, 2, device=backend)
+        ops.prompt_attention(dq, dk, dv, out, _i32([0, n], backend), _i32([0, m], backend), causal=causal, scale=1.0, lse=lse)
+        seen = _seen(n, m, causal)
+        _far_expect(out, scores, seen, v, dt, (top, causal))
+        want = torch.stack([torch.logsumexp(scores[s], 0) for s in seen])
+        assert ((lse.double().cpu() - want[:, None]).abs() <= 2.0 ** -22 * want.abs()[:, None] + 1e-3).all()
+    b = 4                                                           # pieces of a prefix and own keys, joined
+    out = torch.empty(b, 2, d, dtype=dt, device=backend)
+    own_k, own_v = dk[300:].expand(b, 30, 1, d).contiguous(), dv[300:].expand(b, 30, 1, d).contiguous()
+    ops.prefix_attention(dq[:b], dk[:300], dv[:300], own_k, own_v, _i32([30, 1, 17, 0], backend), out, scale=1.0)
+    seen = torch.arange(m) < 300 + torch.tensor([30, 1, 17, 0])[:, None]
+    _far_expect(out, scores, seen, v, dt, (top, "prefix"))
+
+
+@DT
+def test_far_scores_whose_keys_are_shared_by_work_groups(backend, dt):
+    g = torch.Generator().manual_seed(4)
+    n, m, d = 3, 1500, 32
+    assert ops.prompt_splits(1, n, m, 2, 1) > 1
+    q, k, scores = _far_case(dt, 1, 14, 64.0, n, m, d, g)
+    v = torch.randn(m, 1, d, generator=g).to(dt)
+    out = torch.empty(n, 2, d, dtype=dt, device=backend)
+    ops.prompt_attention(q.to(backend), k.to(backend), v.to(backend), out, _i32([0, n], backend), _i32([0, m], backend), scale=1.0)
+    _far_expect(out, scores, _seen(n, m, True), v, dt, "split")
+
+
+@DT
+def test_random_queries_and_keys_of_large_size(backend, dt):
+    """Inputs near the top of f16, 10^6 in the wider types: the softmax of such scores is one key's value unless two meet within rounding."""
+    g = torch.Generator().manual_seed(5)
+    a, n, m, d = (1.5e4 if dt == F16 else 1e6), 48, 140, 64
+    q, k, v = (torch.randn(t, h, d, generator=g) for t, h in ((n, 2), (m, 1), (m, 1)))
+    q, k, v = (q * a).clamp(-4 * a, 4 * a).to(dt), (k * a).clamp(-4 * a, 4 * a).to(dt), v.to(dt)
+    out = torch.empty(n, 2, d, dtype=dt, device=backend)
+    ops.prompt_attention(q.to(backend), k.to(backend), v.to(backend), out, _i32([0, n], backend), _i32([0, m], backend), causal=False)
+    s = (q.double()[:, :, None] * k.double()[None, None, :, 0]).sum(-1) * d ** -0.5
+    best = s.topk(2, -1)
+    slack = (d + 4) * 2.0 ** -24 * (q.double().abs()[:, :, None] * k.double().abs()[None, None, :, 0]).sum(-1).amax(-1) * d ** -0.5
+    clear = best.values[..., 0] - best.values[..., 1] > 2 * slack + 100
+    assert clear.float().mean() > 0.9
+    got = out.float().cpu()
+    assert bool(got.isfinite().all()) and got.abs().max() <= v.float().abs().max() * 1.01
+    assert torch.equal(out.cpu()[clear], v[:, 0][best.indices[..., 0]][clear])
