@@ -8,12 +8,21 @@
 
 namespace pp {
 
+// Sequences up to which keys are shared: each wave of the joining launch looks over their offsets.
+constexpr int kSharedSequences = 4096;
+
+// an offset, inside [0, most]
+__device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
+  const int64_t v = cu[i];
+  return v < 0 ? 0 : v > most ? most : v;
+}
+
 struct PartsK {
   float* o;   // [row][part][D]
   float* ml;  // [row][part][2]
   void* out;  // [b][L][H][D] by strides; row = (b L + token) H + head
   float* lse; // [row] or null
-  const int* cu_q;  // or null: rows of the tokens before cu_q[0] and from cu_q[ncu] on are left as they were
+  const int* cu_q;  // or null: rows of the tokens before cu_q[0] and from cu_q[ncu] on are left as they were, all rows if an offset decreases
   int64_t rows, out_seq, out_row, out_head;
   int L, H, D, parts, ncu;
   float sc, scale;
@@ -87,8 +96,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const PartsK a, int
   sm[tid] = m;
   sl[tid] = l;
   sany[tid] = any;
+  // Every row between the offsets has its parts stored only if they do not decrease (the search for a tile's sequence needs the order); else
+  // scratch that nobody wrote could be among them.
+  bool down = false;
+  if (a.cu_q)
+    for (int i = lane_id(); i < a.ncu; i += 64) down |= clamped(a.cu_q, i, a.L) > clamped(a.cu_q, i + 1, a.L);
+  down = wave_any(down);
   __syncthreads();
-  if (!live || pg != 0) return;
+  if (!live || pg != 0 || down) return;
   float top = m;
   for (int g = 1; g < PG; ++g) top = fmaxf(top, sm[tid + g * DL]);
   const float w = m == top ? 1.f : fast_exp2((m - top) * a.sc);

@@ -10,6 +10,8 @@
 // multiple or divisor of 8) of them a head's keys stay in the L2 of its XCDs.
 // Few tiles with many keys leave most of the chip idle: with `splits` > 1 a tile's keys go to that many work-groups, whose parts a second
 // launch joins (attention_parts.h).
+// The search needs offsets that do not decrease.  Others hit no memory but the tensors': a tile is then taken for the wrong sequence and
+// returns, or takes rows of a sequence that it found, and with splits nothing is joined.
 #include "attention_parts.h"
 
 #include <math.h>
@@ -28,11 +30,6 @@ struct PromptK {
   float scale, sc;
   PartsK parts;
 };
-
-__device__ __forceinline__ int64_t clamped(const int* cu, int i, int64_t most) {
-  const int64_t v = cu[i];
-  return v < 0 ? 0 : v > most ? most : v;
-}
 
 template <typename Tile>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
@@ -193,8 +190,8 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
   a.Tq = p->Tq; a.Tk = p->Tk;
   a.B = (int)p->B; a.H = (int)p->H; a.KH = (int)p->KH; a.G = (int)(p->H / p->KH); a.D = (int)p->D; a.causal = p->causal != 0;
   a.scale = p->scale; a.sc = p->scale * kLog2e;
-  a.splits = splits;
-  if (splits > 1) {
+  a.splits = p->B <= kSharedSequences ? splits : 1;
+  if (a.splits > 1) {
     PartsK& pt = a.parts;
     pt.rows = p->Tq * p->H; pt.L = (int)p->Tq; pt.H = a.H; pt.D = a.D; pt.parts = splits;
     pt.o = (float*)p->scratch;

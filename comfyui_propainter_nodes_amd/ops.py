@@ -1165,11 +1165,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
                      cu_k: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
                      lse: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over packed sequences: q, out [Tq,H,D], k, v [Tk,KH,D] (any strides, dense last dim; f16 / bf16 / fp32), H a multiple of
-    KH; sequence s = query rows cu_q[s]:cu_q[s+1] and key rows cu_k[s]:cu_k[s+1] (i32 on the device; cu_k None: cu_q).  causal: query i of
-    n sees key j of m if j <= i + m - n.  A query without a key gets 0; rows outside every sequence are left as they were.
-    scale: 1/sqrt(D) by default.  lse: fp32 [Tq,H], ln of the softmax sums (-inf without a key).  out may be q (the same view; not for
-    fp32 heads of more than 128 channels); it must not overlap k or v.  `scratch`: float32, prompt_attention_scratch() elements (0 for most calls); by default a tensor of this call's own, so that two
-    captured graphs or two streams never share one.  A caller that passes its own must not let two calls run on it at once."""
+    KH; sequence s = query rows cu_q[s]:cu_q[s+1] and key rows cu_k[s]:cu_k[s+1] (i32 on the device, none below the one before it;
+    cu_k None: cu_q).  causal: query i of n sees key j of m if j <= i + m - n.  A query without a key gets 0; rows outside every sequence
+    are left as they were.  scale: 1/sqrt(D) by default.  lse: fp32 [Tq,H], ln of the softmax sums (-inf without a key).  out may be q (the
+    same view; not for fp32 heads of more than 128 channels); it must not overlap k or v.  `scratch`: float32,
+    prompt_attention_scratch() elements (0 for most calls); by default a tensor of this call's own, so that two captured graphs or two
+    streams never share one.  A caller that passes its own must not let two calls run on it at once."""
     cu_k = cu_q if cu_k is None else cu_k
     check_device(q, k, v, out, cu_q, cu_k, lse)
     qs, ks, vs, os_ = _heads_view("q", q, 3), _heads_view("k", k, 3), _heads_view("v", v, 3), _heads_view("out", out, 3)

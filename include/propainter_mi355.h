@@ -545,7 +545,9 @@ int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p);
  *   out = softmax_j(scale * q . k_j) v_j;  lse (optional) = ln sum_j exp(scale * q . k_j).
  * A query that sees no key gets out = 0, lse = -inf.  Query rows outside every sequence are not written.  Keys, values and queries
  * that a row does not see never reach its result, whatever they hold (NaN and infinities included).
- * The offsets live on the device: values outside [0, Tq] / [0, Tk] are clamped, a sequence of negative length is empty.
+ * The offsets live on the device.  They must not decrease.  Values outside [0, Tq] / [0, Tk] are clamped; where cu_k decreases the sequence
+ * has no key; where cu_q decreases, the call touches nothing but its tensors, and which rows are written is not specified (a row in
+ * one sequence only is left as it was or holds its result).
  * Strides in elements, those of key and value rows below 2^24; the last dim is dense; every row start is 16-byte aligned;
  * D % 8 == 0 (% 4 for PP_F32), D <= 256.
  * out may be q (same strides; not for PP_F32 with D > 128), and overlaps nothing else.
@@ -568,7 +570,7 @@ typedef struct {
   const void* cu_k; /* i32 [B + 1] */
   int64_t B, Tq, Tk, H, KH, D;
   float scale; /* > 0, finite */
-  int32_t splits; /* work-groups that share the keys of a tile of rows (0 = 1): for few rows with many keys */
+  int32_t splits; /* work-groups that share the keys of a tile of rows (0 = 1): for few rows with many keys; 1 above 4096 sequences */
   void* scratch;  /* splits > 1: caller-owned, 16-byte aligned, Tq * H * splits * (D + 4) floats */
   int64_t scratch_bytes;
 } pp_prompt_attention_params;

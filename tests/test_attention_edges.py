@@ -171,3 +171,57 @@ def test_random_queries_and_keys_of_large_size(backend, dt):
     got = out.float().cpu()
     assert bool(got.isfinite().all()) and got.abs().max() <= v.float().abs().max() * 1.01
     assert torch.equal(out.cpu()[clear], v[:, 0][best.indices[..., 0]][clear])
+
+
+# --------------------------------------------------------------------------------------------
+# offsets that decrease (device data: no host check sees them)
+# --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cu_q,cu_k", [
+    ([0, 400, 10, 10], [0, 400, 400, 400]),         # one work-group per tile
+    ([0, 390, 10, 400], [0, 800, 1600, 2400]),      # shared keys, in this case and those below
+    ([10, 0, 400], [0, 1200, 2400]),
+    ([0, 200, 150, 400], [0, 2400, 2400, 2400]),
+    ([400, 200, 0], [0, 1200, 2400]),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_offsets_that_decrease(backend, cu_q, cu_k, causal):
+    """Such a call is not specified, but a row is left as it was or holds the result of a sequence that contains it, never what the scratch
+    held."""
+    g = torch.Generator().manual_seed(6)
+    tq, d, m = 400, 32, cu_k[-1]
+    q, k, v = (torch.randn(n, 1, d, generator=g) for n in (tq, m, m))
+    dq, dk, dv = q.to(backend), k.to(backend), v.to(backend)
+    out = torch.full((tq, 1, d), 7.0, device=backend)
+    dcu = _i32(cu_q, backend)
+    need = ops.prompt_attention_scratch(dq, dk, dcu)
+    assert (need > 0) == (m == 2400)
+    scratch = torch.full((max(1, need),), math.nan, device=backend)
+    ops.prompt_attention(dq, dk, dv, out, dcu, _i32(cu_k, backend), causal=causal, scratch=scratch)
+    out = out.cpu()[:, 0]
+    fine = (out == 7.0).all(-1)
+    for a, b, c, e in zip(cu_q, cu_q[1:], cu_k, cu_k[1:]):
+        if b > a:
+            s = (q[a:b, 0].double() @ k[c:e, 0].double().T * d ** -0.5).masked_fill(~_seen(b - a, e - c, causal), -INF)
+            w, vv = torch.nan_to_num(torch.softmax(s, -1)), v[c:e, 0].double()
+            smax = (q[a:b, 0].abs() @ k[c:e, 0].abs().T).max().item() * d ** -0.5 if e > c else 0.0
+            fine[a:b] |= ((out[a:b].double() - w @ vv).abs() <= _attn_tol(F32, w @ vv, w @ vv.abs(), e - c, d, smax, _vmax(v))).all(-1)
+    assert bool(fine.all()), (~fine).nonzero()[:, 0].tolist()
+
+
+def test_many_sequences_do_not_share_keys(emu_lib):
+    """`splits` is a hint: with more sequences than the joining launch can look over the keys of a tile stay with one work-group."""
+    g = torch.Generator().manual_seed(7)
+    n, d = 5000, 8
+    q, k, v = (torch.randn(n, 1, d, generator=g) for _ in range(3))
+    cu = torch.arange(n + 1, dtype=torch.int32)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    ops.prompt_attention(q, k, v, want, cu)
+    scratch = torch.full((n * 2 * (d + 4),), math.nan)
+    P = lib.STRUCTS["pp_prompt_attention_params"]()
+    P.dtype, P.causal, P.scale, P.splits = lib.CONSTS["PP_F32"], 1, d ** -0.5, 2
+    P.q, P.k, P.v, P.out, P.cu_q, P.cu_k = (t.data_ptr() for t in (q, k, v, out, cu, cu))
+    P.q_row = P.k_row = P.v_row = P.out_row = d
+    P.B, P.Tq, P.Tk, P.H, P.KH, P.D = n, n, n, 1, 1, d
+    P.scratch, P.scratch_bytes = scratch.data_ptr(), scratch.numel() * 4
+    emu_lib.call("pp_prompt_attention", 0, P)
+    assert torch.equal(out, want) and bool(scratch.isnan().all())
