@@ -152,8 +152,9 @@ extern "C" int32_t pp_prefix_attention(void* stream, const pp_prefix_attention_p
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: H must be a multiple of KH");
   const int e = p->dtype == PP_F32 ? 4 : 8;  // elements of 16 bytes
   if (p->D < 1 || p->D > 256 || p->D % e) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: D must be a multiple of 8 (fp32: 4) up to 256");
-  if (p->B < 0 || p->L < 0 || p->P < 0 || p->S < 0 || p->B > (1 << 24) || p->L > (1 << 20) || p->P > INT32_MAX || p->S > INT32_MAX)
+  if (p->B < 0 || p->L < 0 || p->P < 0 || p->S < 0 || p->B > (1 << 24) || p->L > (1 << 20))
     return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: B, L, P, S out of range");
+  if (p->P > kMostKeys || p->S > kMostKeys) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prefix_attention: P or S above 2^31 - 1024");
   if ((p->P > 0 && (!p->kp || !p->vp)) || (p->S > 0 && (!p->ko || !p->vo))) return pp_fail(PP_ERR_BAD_ARG, "pp_prefix_attention: null keys or values");
   if (p->prefix_splits < 0 || p->own_splits < 0 || p->prefix_splits > 65536 || p->own_splits > 65536 || (p->P > 0 && p->prefix_splits < 1) ||
       (p->S > 0 && p->own_splits < 1) || p->prefix_splits + p->own_splits < 1)

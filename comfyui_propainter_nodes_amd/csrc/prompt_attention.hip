@@ -162,8 +162,9 @@ extern "C" int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_p
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: H must be a multiple of KH");
   const int e = p->dtype == PP_F32 ? 4 : 8;  // elements of 16 bytes
   if (p->D < 1 || p->D > 256 || p->D % e) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: D must be a multiple of 8 (fp32: 4) up to 256");
-  if (p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->B > INT32_MAX / 2 || p->Tq > INT32_MAX || p->Tk > INT32_MAX)
+  if (p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->B > INT32_MAX / 2 || p->Tq > INT32_MAX)
     return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: B, Tq, Tk must be in [0, 2^31)");
+  if (p->Tk > kMostKeys) return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: Tk above 2^31 - 1024");
   if (p->Tq * p->H > (int64_t)1 << 40 || p->B * p->KH > (int64_t)1 << 32)  // (what is computed from them stays inside 64 bits)
     return pp_fail(PP_ERR_UNSUPPORTED, "pp_prompt_attention: Tq * H or B * KH too large");
   if (!(p->scale > 0.f) || !(p->scale * kLog2e < INFINITY)) return pp_fail(PP_ERR_BAD_ARG, "pp_prompt_attention: scale must be positive and finite");

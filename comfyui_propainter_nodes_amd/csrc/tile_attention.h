@@ -38,6 +38,8 @@ namespace pp {
 
 constexpr float kMost = 4096.f;
 constexpr float kFar = 4096.f;  // |m sc| from which a block is not weighed by 2^(s sc - m sc)
+// Keys of one walk: its counters are 32 bits wide and run up to three blocks past the last key.
+constexpr int64_t kMostKeys = ((int64_t)1 << 31) - 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 #ifdef PP_EMU

@@ -549,7 +549,7 @@ int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p);
  * has no key; where cu_q decreases, the call touches nothing but its tensors, and which rows are written is not specified (a row in
  * one sequence only is left as it was or holds its result).
  * Strides in elements, those of key and value rows below 2^24; the last dim is dense; every row start is 16-byte aligned;
- * D % 8 == 0 (% 4 for PP_F32), D <= 256.
+ * D % 8 == 0 (% 4 for PP_F32), D <= 256; Tk <= 2^31 - 1024.
  * out may be q (same strides; not for PP_F32 with D > 128), and overlaps nothing else.
  * PP_F16 / PP_BF16: MFMA operands in the storage type (the probabilities are rounded to it once, as operands of the second
  * product), fp32 scores, sums and accumulators.  PP_F32: everything fp32 (f32 MFMA).
@@ -585,7 +585,7 @@ int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p);
  * The prefix's keys and values are read once for all rows of a key / value head, not once per sequence.
  * `scratch`: caller-owned, 16-byte aligned, B * L * H * (prefix_splits + own_splits) * (D + 4) floats; prefix_splits pieces of the
  * prefix and own_splits pieces of each own range go to different work-groups and are joined in a fixed order (both >= 0, a
- * part with keys needs at least one).  Strides in elements as in pp_prompt_attention.
+ * part with keys needs at least one).  Strides in elements as in pp_prompt_attention; P, S <= 2^31 - 1024.
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   int32_t dtype; /* q, kp, vp, ko, vo, out: PP_F32, PP_F16 or PP_BF16 */

@@ -225,3 +225,44 @@ def test_many_sequences_do_not_share_keys(emu_lib):
     P.scratch, P.scratch_bytes = scratch.data_ptr(), scratch.numel() * 4
     emu_lib.call("pp_prompt_attention", 0, P)
     assert torch.equal(out, want) and bool(scratch.isnan().all())
+
+
+# --------------------------------------------------------------------------------------------
+# lengths at the end of the accepted range
+# --------------------------------------------------------------------------------------------
+def _prompt_params(cu_k, tk, t):
+    P = lib.STRUCTS["pp_prompt_attention_params"]()
+    P.dtype, P.causal, P.scale = lib.CONSTS["PP_F32"], 0, 1.0
+    P.q, P.k, P.v, P.out = (x.data_ptr() for x in t[:4])
+    P.cu_q, P.cu_k = t[4].data_ptr(), cu_k.data_ptr()
+    P.q_row = P.k_row = P.v_row = P.out_row = 8
+    P.B, P.Tq, P.Tk, P.H, P.KH, P.D = 1, 1, tk, 1, 1, 8
+    return P
+
+
+def test_lengths_that_a_walk_over_the_keys_cannot_count(emu_lib):
+    """Keys are counted in 32 bits, up to three blocks beyond the last: lengths above 2^31 - 1024 are refused.  (No such tensor is made: the
+    offsets and lengths of the accepted calls leave one key.)"""
+    t = (torch.ones(1, 8), torch.ones(1, 8), torch.full((1, 8), 3.0), torch.zeros(1, 8), torch.tensor([0, 1], dtype=torch.int32))
+    cu_k = torch.tensor([0, 1], dtype=torch.int32)
+    for tk in (2 ** 31 - 1, 2 ** 31 - 1023):
+        with pytest.raises(RuntimeError, match="2\\^31 - 1024"):
+            emu_lib.call("pp_prompt_attention", 0, _prompt_params(cu_k, tk, t))
+    emu_lib.call("pp_prompt_attention", 0, _prompt_params(cu_k, 2 ** 31 - 1024, t))
+    assert bool((t[3] == 3).all())
+    scratch, own_len = torch.zeros(4 * 12), torch.ones(1, dtype=torch.int32)
+    for p, s in ((2 ** 31 - 1, 0), (2 ** 31 - 1023, 0), (0, 2 ** 31 - 1023), (0, 2 ** 31 - 1024)):
+        P = lib.STRUCTS["pp_prefix_attention_params"]()
+        P.dtype, P.scale = lib.CONSTS["PP_F32"], 1.0
+        P.q, P.kp, P.vp, P.ko, P.vo, P.out = (t[i].data_ptr() for i in (0, 1, 2, 1, 2, 3))
+        P.own_len, P.scratch, P.scratch_bytes = own_len.data_ptr(), scratch.data_ptr(), scratch.numel() * 4
+        P.kp_row = P.vp_row = P.ko_row = P.vo_row = 8
+        P.prefix_splits, P.own_splits = int(p > 0), int(s > 0)
+        P.B, P.L, P.P, P.S, P.H, P.KH, P.D = 1, 1, p, s, 1, 1, 8
+        if s == 2 ** 31 - 1024:
+            t[3].zero_()
+            emu_lib.call("pp_prefix_attention", 0, P)
+            assert bool((t[3] == 3).all())
+        else:
+            with pytest.raises(RuntimeError, match="2\\^31 - 1024"):
+                emu_lib.call("pp_prefix_attention", 0, P)
