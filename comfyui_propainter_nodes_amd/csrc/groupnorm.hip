@@ -201,21 +201,23 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+constexpr int kFinishBlocks = 2048;  // 8 work-groups per CU; more (image, group) pairs than they have waves go round again
+
 // a wave per (image, group): its lanes share the chunks
 __global__ void __launch_bounds__(256) groupnorm_finish_kernel(const GroupNormK k) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (int64_t)k.N * k.G) return;
-  const int64_t n = i / k.G, g = i - n * k.G;
-  const double* src = k.partials + (n * k.nchunks * k.G + g) * 2;
-  double s = 0.0, q = 0.0;
-  for (int c = lane_id(); c < k.nchunks; c += 64) {
-    s += src[(int64_t)c * k.G * 2];
-    q += src[(int64_t)c * k.G * 2 + 1];
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < (int64_t)k.N * k.G; i += (int64_t)gridDim.x * 4) {
+    const int64_t n = i / k.G, g = i - n * k.G;
+    const double* src = k.partials + (n * k.nchunks * k.G + g) * 2;
+    double s = 0.0, q = 0.0;
+    for (int c = lane_id(); c < k.nchunks; c += 64) {
+      s += src[(int64_t)c * k.G * 2];
+      q += src[(int64_t)c * k.G * 2 + 1];
+    }
+    s = wave_sum(s);
+    q = wave_sum(q);
+    if (lane_id() == 0)
+      reinterpret_cast<f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2)[i] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
   }
-  s = wave_sum(s);
-  q = wave_sum(q);
-  if (lane_id() == 0)
-    reinterpret_cast<f4*>(k.partials + (int64_t)k.N * k.nchunks * k.G * 2)[i] = finish_stats(s, q, (double)k.HW * k.cpg, k.eps);
 }
 
 // What a vector of V channels needs: ((x - mh) - ml) a + b; with 16-bit storage x - mh is exact to 2^-24 of the larger one and -ml a goes
@@ -371,7 +373,8 @@ static int launch_groupnorm_act(void* stream, pp::GroupNormK& k) {
   int rc = pp_check_launch("pp_groupnorm(sums)");
   if (rc != PP_OK) return rc;
   if (!k.join) {
-    PP_LAUNCH(groupnorm_finish_kernel, dim3((unsigned)(((int64_t)k.N * k.G + 3) / 4)), dim3(256), 0, stream, k);
+    const int64_t blocks = ((int64_t)k.N * k.G + 3) / 4;
+    PP_LAUNCH(groupnorm_finish_kernel, dim3((unsigned)(blocks < kFinishBlocks ? blocks : kFinishBlocks)), dim3(256), 0, stream, k);
     rc = pp_check_launch("pp_groupnorm(finish)");
     if (rc != PP_OK) return rc;
   }
