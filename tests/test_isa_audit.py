@@ -69,3 +69,16 @@ def test_no_packed_fp32_instruction_swaps_operand_halves():
     r = S.audit_packed_f32_op_sel()
     assert r["kernels"] >= 150, r["kernels"]
     assert not r["violations"], r["violations"][:10]
+
+
+def test_no_packed_fp32_instruction_of_any_form():
+    """build_hip() switches the target feature off, so the broadcast forms that the explicit f4 arithmetic would use are gone as well."""
+    import shipped_isa as S
+
+    from comfyui_propainter_nodes_amd import build
+
+    if not S.tools_available():
+        pytest.skip("no llvm-objcopy / llvm-objdump")
+    build.build_hip()
+    r = S.audit_packed_f32_op_sel()
+    assert r["kernels"] >= 150 and r["packed_fp32"] == 0, r
