@@ -29,7 +29,7 @@ struct PartsK {
 };
 
 template <typename Tile>
-__device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const AttnState<Tile>& st, int rb, int64_t row, int part, bool any, int d0,
+__device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const AttnState<Tile>& st, int64_t row, int part, bool any, int d0,
                                            int DV) {  // channels d0 .. d0 + DV - 1
   const int64_t at = row * a.parts + part;
   float* dst = a.o + at * a.D + d0;
@@ -38,12 +38,12 @@ __device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * db + 8 * g + 4 * t.h;
-      const f16v& o = st.o[rb][db];
+      const f16v& o = st.o[db];
       if (d < DV) *reinterpret_cast<f4*>(dst + d) = f4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
     }
   if (t.h == 0 && d0 == 0) {
-    a.ml[2 * at] = st.m[rb];
-    a.ml[2 * at + 1] = any ? st.l[rb] : -1.f;
+    a.ml[2 * at] = st.m;
+    a.ml[2 * at + 1] = any ? st.l : -1.f;
   }
 }
 

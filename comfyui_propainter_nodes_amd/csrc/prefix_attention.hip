@@ -31,7 +31,7 @@ struct PrefixK {
 template <typename Tile>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention_kernel(const PrefixK a) {
   typedef typename Tile::type T;
-  constexpr int kRows = Tile::kRows, RB = Tile::RB;
+  constexpr int kRows = Tile::kRows;
   const int lane = lane_id(), wave = wave_uniform((int)threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
   const int d0 = (int)blockIdx.x % Tile::kHalves * Tile::kDV;  // the value channels from d0 on
   const int DV = a.D - d0 < Tile::kDV ? a.D - d0 : Tile::kDV;
@@ -78,34 +78,27 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prefix_attention
     const int64_t c = shared ? n1 - n0 : visible - a.L + row / a.G + 1 - n0;
     return (int)(c < 0 ? 0 : c > n1 - n0 ? n1 - n0 : c);
   };
-  const int64_t last = rows - 1, wrow = row0 + 32 * RB * wave;
-  AttnLimits<RB> lim;
-  lim.wave_min = wrow <= last ? limit_of(wrow) : 0;
-  lim.wave_max = wrow <= last ? limit_of(wrow + 32 * RB - 1 < last ? wrow + 32 * RB - 1 : last) : 0;
+  const int64_t last = rows - 1, wrow = row0 + 32 * wave, row = wrow + q32;
+  AttnLimits lim;
+  lim.wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
   lim.group_min = limit_of(row0);
   lim.nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
   Tile t;
   AttnState<Tile> st;
   t.init(PP_DYN_SMEM);
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int64_t row = wrow + 32 * rb + q32;
-    const bool live = row <= last;
-    lim.row[rb] = live ? limit_of(row) : 0;
+  const bool live = row <= last;
+  lim.row = live ? limit_of(row) : 0;
+  {
     const int64_t b = shared ? row / lg : seq;
     const int in_seq = (int)(shared ? row % lg : row);
-    t.load_q(rb, live ? (const T*)a.q + b * a.q_seq + (in_seq / a.G) * a.q_row + (kh * a.G + in_seq % a.G) * a.q_head : nullptr, a.D);
+    t.load_q(live ? (const T*)a.q + b * a.q_seq + (in_seq / a.G) * a.q_row + (kh * a.G + in_seq % a.G) * a.q_head : nullptr, a.D);
   }
   attend(t, st, k + n0 * k_row, v + n0 * v_row, k_row, v_row, lim, a.D, DV, a.sc);
   if (st.not_finite) add_not_finite(t, st, v + n0 * v_row, v_row, lim, DV);
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int64_t row = wrow + 32 * rb + q32;
-    if (row > last) continue;
-    const int64_t b = shared ? row / lg : seq;
-    const int in_seq = (int)(shared ? row % lg : row);
-    store_part(a.parts, t, st, rb, (b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G, part, lim.row[rb] > 0, d0, DV);
-  }
+  if (!live) return;
+  const int64_t b = shared ? row / lg : seq;
+  const int in_seq = (int)(shared ? row % lg : row);
+  store_part(a.parts, t, st, (b * a.L + in_seq / a.G) * a.H + kh * a.G + in_seq % a.G, part, lim.row > 0, d0, DV);
 }
 
 }  // namespace pp
@@ -130,17 +123,17 @@ template <typename T>
 static int launch_prefix_d(void* stream, pp::PrefixK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
-    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 1, 2>>(stream, a);
-    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 1, 2>>(stream, a);
-    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1, 1>>(stream, a);
-    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1, 1>>(stream, a);
-    return launch_prefix<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 2>>(stream, a);
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 2>>(stream, a);
+    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1>>(stream, a);
+    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1>>(stream, a);
+    return launch_prefix<AttnTile<T, 256, 4, 1>>(stream, a);
   } else {
-    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 1, 1>>(stream, a);
-    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 1, 1>>(stream, a);
-    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1, 1>>(stream, a);
-    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1, 1>>(stream, a);
-    return launch_prefix<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+    if (a.D <= 32) return launch_prefix<AttnTile<T, 32, 4, 1>>(stream, a);
+    if (a.D <= 64) return launch_prefix<AttnTile<T, 64, 4, 1>>(stream, a);
+    if (a.D <= 96) return launch_prefix<AttnTile<T, 96, 4, 1>>(stream, a);
+    if (a.D <= 128) return launch_prefix<AttnTile<T, 128, 4, 1>>(stream, a);
+    return launch_prefix<AttnTile<T, 256, 4, 1>>(stream, a);
   }
 }
 

@@ -34,7 +34,7 @@ struct PromptK {
 template <typename Tile>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention_kernel(const PromptK a) {
   typedef typename Tile::type T;
-  constexpr int kRows = Tile::kRows, RB = Tile::RB;
+  constexpr int kRows = Tile::kRows;
   const int id = (int)blockIdx.x / Tile::kHalves, d0 = (int)blockIdx.x % Tile::kHalves * Tile::kDV;  // the value channels from d0 on
   const int DV = a.D - d0 < Tile::kDV ? a.D - d0 : Tile::kDV;
   const int kh = id % a.KH, split = id / a.KH % a.splits;
@@ -63,55 +63,46 @@ __global__ void __launch_bounds__(Tile::kThreads, Tile::kWaves) prompt_attention
     const int64_t c = (a.causal ? row / a.G + 1 + m - n : m) - first;
     return (int)(c < 0 ? 0 : c > most ? most : c);
   };
-  const int64_t last = rows - 1, wrow = row0 + 32 * RB * wave;
+  const int64_t last = rows - 1, wrow = row0 + 32 * wave, row = wrow + q32;
   if (a.splits > 1) {
     const int all = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
     const int per = ((all + a.splits - 1) / a.splits + 63) / 64 * 64;
     first = split * per < all ? split * per : all;
     most = all - first < per ? all - first : per;
   }
-  AttnLimits<RB> lim;
-  lim.wave_min = wrow <= last ? limit_of(wrow) : 0;
-  lim.wave_max = wrow <= last ? limit_of(wrow + 32 * RB - 1 < last ? wrow + 32 * RB - 1 : last) : 0;
+  AttnLimits lim;
+  lim.wave_max = wrow <= last ? limit_of(wrow + 31 < last ? wrow + 31 : last) : 0;
   lim.group_min = limit_of(row0);
   lim.nkeys = limit_of(row0 + kRows - 1 < last ? row0 + kRows - 1 : last);
   Tile t;
   AttnState<Tile> st;
   t.init(PP_DYN_SMEM);
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int64_t row = wrow + 32 * rb + q32;
-    const bool live = row <= last;
-    lim.row[rb] = live ? limit_of(row) : 0;
-    t.load_q(rb, live ? (const T*)a.q + (q0 + row / a.G) * a.q_row + (kh * a.G + row % a.G) * a.q_head : nullptr, a.D);
-  }
+  const bool live = row <= last;
+  lim.row = live ? limit_of(row) : 0;
+  t.load_q(live ? (const T*)a.q + (q0 + row / a.G) * a.q_row + (kh * a.G + row % a.G) * a.q_head : nullptr, a.D);
   const T* k = (const T*)a.k + (k0 + first) * a.k_row + kh * a.k_head;
   const T* v = (const T*)a.v + (k0 + first) * a.v_row + kh * a.v_head + d0;
   attend(t, st, k, v, a.k_row, a.v_row, lim, a.D, DV, a.sc);
   if (st.not_finite) add_not_finite(t, st, v, a.v_row, lim, DV);
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int64_t row = wrow + 32 * rb + q32;
-    if (row > last) continue;
-    const int64_t token = q0 + row / a.G;
-    const int head = kh * a.G + (int)(row % a.G);
-    if (a.splits > 1) {
-      store_part(a.parts, t, st, rb, token * a.H + head, split, lim.row[rb] > 0, d0, DV);
-      continue;
-    }
-    // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
-    const float inv = lim.row[rb] > 0 ? 1.f / st.l[rb] : 0.f;
-    T* dst = (T*)a.out + token * a.out_row + head * a.out_head + d0;
-#pragma unroll
-    for (int db = 0; db < Tile::kDB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * db + 8 * g + 4 * h;
-        const f16v& o = st.o[rb][db];
-        if (d < DV) Tile::store4(dst + d, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
-      }
-    if (a.lse && h == 0 && d0 == 0) a.lse[token * a.H + head] = lim.row[rb] > 0 ? st.m[rb] * a.scale + logf(st.l[rb]) : neg_inf();
+  if (!live) return;
+  const int64_t token = q0 + row / a.G;
+  const int head = kh * a.G + (int)(row % a.G);
+  if (a.splits > 1) {
+    store_part(a.parts, t, st, token * a.H + head, split, lim.row > 0, d0, DV);
+    return;
   }
+  // no key at all: 0; keys whose scores are all -inf: 0 / 0, as the formula says
+  const float inv = lim.row > 0 ? 1.f / st.l : 0.f;
+  T* dst = (T*)a.out + token * a.out_row + head * a.out_head + d0;
+#pragma unroll
+  for (int db = 0; db < Tile::kDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * db + 8 * g + 4 * h;
+      const f16v& o = st.o[db];
+      if (d < DV) Tile::store4(dst + d, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
+    }
+  if (a.lse && h == 0 && d0 == 0) a.lse[token * a.H + head] = lim.row > 0 ? st.m * a.scale + logf(st.l) : neg_inf();
 }
 
 }  // namespace pp
@@ -132,25 +123,25 @@ template <typename T>
 static int launch_prompt_d(void* stream, pp::PromptK& a) {
   using namespace pp;
   if constexpr (sizeof(T) == 2) {
-    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 1, 2>>(stream, a);
-    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 1, 2>>(stream, a);
-    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1, 1>>(stream, a);
-    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1, 1>>(stream, a);
-    return launch_prompt<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 2>>(stream, a);
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 2>>(stream, a);
+    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1>>(stream, a);
+    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1>>(stream, a);
+    return launch_prompt<AttnTile<T, 256, 4, 1>>(stream, a);
   } else {
     // Rows of a sequence that fit one 64-row work-group of 2 waves: with 4 waves half of them would idle (45 rows and keys, 128 channels: 153
     // -> 133 us for 2592 sequences and heads).  Long sequences share the staging of 4 waves (2048 tokens: 277 us against 424).
     if (a.Tq * a.G <= 64 * (int64_t)a.B) {
-      if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 2, 1, 1>>(stream, a);
-      if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 1, 1>>(stream, a);
-      if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 2, 1, 1>>(stream, a);
-      if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 2, 1, 1>>(stream, a);
+      if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 2, 1>>(stream, a);
+      if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 1>>(stream, a);
+      if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 2, 1>>(stream, a);
+      if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 2, 1>>(stream, a);
     }
-    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 1, 1>>(stream, a);
-    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 1, 1>>(stream, a);
-    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1, 1>>(stream, a);
-    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1, 1>>(stream, a);
-    return launch_prompt<AttnTile<T, 256, 4, 1, 1>>(stream, a);
+    if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 4, 1>>(stream, a);
+    if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 4, 1>>(stream, a);
+    if (a.D <= 96) return launch_prompt<AttnTile<T, 96, 4, 1>>(stream, a);
+    if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1>>(stream, a);
+    return launch_prompt<AttnTile<T, 256, 4, 1>>(stream, a);
   }
 }
 

@@ -1,6 +1,6 @@
 // tile_attention.h -- one work-group's attention over a run of keys: the part that pp_prompt_attention and pp_prefix_attention share.
 //
-// A work-group of NW waves takes 32 RB NW query rows, 32 RB per wave, of ONE key / value head (the query heads of a group are rows of the
+// A work-group of NW waves takes 32 NW query rows, 32 per wave, of ONE key / value head (the query heads of a group are rows of the
 // same tile, so their keys are staged once).  Keys are walked in steps of 32 NS through LDS:
 //   S^T = K . Q^T     32x32 MFMA; lane l holds the scores of query l & 31 against keys (r & 3) + 8 (r >> 2) + 4 (l >> 5), r = 0..15
 //   online softmax    lane-local, one exchange between lanes l and l ^ 32; fp32 maxima, sums and accumulators
@@ -21,7 +21,7 @@
 //
 // Bound by the matrix pipes: one causal prompt of 8192 tokens, 32 query heads over 8 key heads of 128, f16: 533-590 us by card, 0.93-1.03 PF/s, MFMA busy
 // 52 % of the cycles at the 1.87 GHz that the card holds under it, LDS 39 %, no bank conflict; 843 TF/s at 64 channels, 860 at 256, f32 136 TF/s
-// (full f32 MFMA rate 157).  RB is 1 everywhere: 64 rows a wave halve the LDS reads, but leave one wave per SIMD and cost register moves (935 us).
+// (full f32 MFMA rate 157).  64 rows a wave would halve the LDS reads, but left one wave per SIMD and cost register moves (935 us).
 // With a maximum per block and per-lane addresses the same call took 703 us, with the MFMAs left to the compiler's order 634.
 //
 // Rows that see different numbers of keys: `limit` is the row's own count, scores at or past it become -inf before the softmax.  Their
@@ -135,12 +135,12 @@ __device__ __forceinline__ int score_key(int r, int h) { return (r & 3) + 8 * (r
 // 16-bit storage.  The two K and two V slots of 32 NS keys lie in LDS row by row, kPitch bytes a row, their 16-byte pieces XOR-swizzled so
 // that the K reads (16 bytes of 32 rows at once) and the transposing V reads (64 bytes of 4 rows at once) touch every bank once.
 // ----------------------------------------------------------------------------------------
-template <typename T, int DP, int NW_, int RB_, int NS_>
+template <typename T, int DP, int NW_, int NS_>
 struct AttnTile {
   typedef T type;
-  static constexpr int NW = NW_, RB = RB_, NS = NS_, kThreads = 64 * NW, kBN = 32 * NS, kRows = 32 * NW * RB;
+  static constexpr int NW = NW_, NS = NS_, kThreads = 64 * NW, kBN = 32 * NS, kRows = 32 * NW;
   static constexpr bool kSteady = true;  // has products(): the pipelined step
-  static constexpr int kWaves = RB > 1 || DP > 128 ? 1 : 2;  // per SIMD
+  static constexpr int kWaves = DP > 128 ? 1 : 2;  // per SIMD
   static constexpr int kPitch = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
   static constexpr int kPieces = DP / 8, kPer = 8, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = DP / 32, kQF = DP / 16;
   static constexpr int kHalves = 1, kDV = DP, kPiecesV = kPieces, kAllV = kAll, kStageV = kStage;
@@ -149,7 +149,7 @@ struct AttnTile {
     h8 f[2];
   };
 
-  h8 q[RB][kQF];
+  h8 q[kQF];
   u4 ks[kStage], vs[kStageV];  // blocks on their way
   unsigned char* smem;
   int q32, h;
@@ -167,32 +167,29 @@ struct AttnTile {
     q32 = (int)threadIdx.x & 31;
     h = ((int)threadIdx.x >> 5) & 1;
   }
-  // row: this lane's query of row block rb, or null
-  __device__ __forceinline__ void load_q(int rb, const T* row, int D) {
+  // row: this lane's query, or null
+  __device__ __forceinline__ void load_q(const T* row, int D) {
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
       const int d = 16 * c + 8 * h;
       u4 v = {0u, 0u, 0u, 0u};
       if (row && d < D) v = *reinterpret_cast<const u4*>(row + d);
-      q[rb][c] = __builtin_bit_cast(h8, v);
+      q[c] = __builtin_bit_cast(h8, v);
     }
   }
   __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + k_at(slot, row, piece)) = ks[i]; }
   __device__ __forceinline__ void store_v(int slot, int i, int row, int piece) const { *reinterpret_cast<u4*>(smem + v_at(slot, row, piece)) = vs[i]; }
-  __device__ __forceinline__ void qk(int slot, f16v (*s)[NS]) const {
+  __device__ __forceinline__ void qk(int slot, f16v* s) const {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[rb][sub][r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[sub][r] = 0.f;
 #pragma unroll
     for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
       for (int c = 0; c < kQF; ++c) {
         const h8 a = *reinterpret_cast<const h8*>(smem + k_at(slot, 32 * sub + q32, 2 * c + h));
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb][sub] = Op<T>::mfma(a, q[rb][c], s[rb][sub]);
+        s[sub] = Op<T>::mfma(a, q[c], s[sub]);
       }
   }
   static __device__ __forceinline__ P pack_p(const float* p) {
@@ -215,43 +212,39 @@ struct AttnTile {
     return h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
   // keys: wave-uniform; sub-tiles behind the last one that any row sees are left out
-  __device__ __forceinline__ void pv(int slot, const P (*p)[NS], f16v (*o)[kDB], int keys) const {
+  __device__ __forceinline__ void pv(int slot, const P* p, f16v* o, int keys) const {
 #pragma unroll
     for (int sub = 0; sub < NS; ++sub) {
       if (sub > 0 && 32 * sub >= keys) break;
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int db = 0; db < kDB; ++db) {
-          const h8 a = v_frag(slot, sub, db, m);
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) o[rb][db] = Op<T>::mfma(a, p[rb][sub].f[m], o[rb][db]);
-        }
+        for (int db = 0; db < kDB; ++db) o[db] = Op<T>::mfma(v_frag(slot, sub, db, m), p[sub].f[m], o[db]);
     }
   }
   // A whole step: w = K Q^T, o += V^T z, y = exp2(x sc + nm) with its sums in bs.  The MFMAs are laid out one fragment at a time, each
   // followed by its share of the exponentials, and the LDS reads run kAhead fragments ahead: left to itself the compiler puts all the vector
   // work behind the last MFMA, and waits for each read.
-  __device__ __forceinline__ void products(int slot, f16v (&w)[RB][NS], const P (&z)[RB][NS], f16v (*o)[kDB], const f16v (&x)[RB][NS],
-                                           P (&y)[RB][NS], const float* nm, float sc, float* bs) const {
+  __device__ __forceinline__ void products(int slot, f16v (&w)[NS], const P (&z)[NS], f16v* o, const f16v (&x)[NS], P (&y)[NS], float nm, float sc,
+                                           float& bs) const {
     constexpr int n1 = NS * kQF, n2 = NS * 2 * kDB, n = n1 + n2, kAhead = 3, kRing = kAhead + 1;
-    constexpr int kEl = RB * NS * 16;
+    constexpr int kEl = NS * 16;
     h8 ring[kRing];
     auto fragment = [&](int j) __attribute__((always_inline)) -> h8 {
       if (j < n1) return *reinterpret_cast<const h8*>(smem + k_at(slot, 32 * (j / kQF) + q32, 2 * (j % kQF) + h));
       const int i = j - n1;
       return v_frag(slot, i / (2 * kDB), i % kDB, i / kDB % 2);
     };
-    u4 yw[RB][NS][2];
+    u4 yw[NS][2];
     float v[kEl];
     auto take = [&](int e) __attribute__((always_inline)) {  // one exponential behind: its result is not waited for
-      const int rb = e / (16 * NS), sub = e / 16 % NS, r = e % 16;
-      bs[rb] = e % (16 * NS) == 0 ? v[e] : bs[rb] + v[e];
-      pin(bs[rb]);
+      const int sub = e / 16, r = e % 16;
+      bs = e == 0 ? v[e] : bs + v[e];
+      pin(bs);
       if (r % 2) {
         unsigned two = Op<T>::pack(v[e - 1], v[e]);
         pin(two);
-        yw[rb][sub][r / 8][r % 8 / 2] = two;
+        yw[sub][r / 8][r % 8 / 2] = two;
       }
     };
 #pragma unroll
@@ -260,31 +253,25 @@ struct AttnTile {
     for (int j = 0; j < n; ++j) {
       if (j + kAhead < n) ring[(j + kAhead) % kRing] = fragment(j + kAhead);
       const h8 a = ring[j % kRing];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        if (j < n1) {
-          const f16v zero = {};
-          w[rb][j / kQF] = Op<T>::mfma(a, q[rb][j % kQF], j % kQF == 0 ? zero : w[rb][j / kQF]);
-        } else {
-          const int i = j - n1;
-          o[rb][i % kDB] = Op<T>::mfma(a, z[rb][i / (2 * kDB)].f[i / kDB % 2], o[rb][i % kDB]);
-        }
+      if (j < n1) {
+        const f16v zero = {};
+        w[j / kQF] = Op<T>::mfma(a, q[j % kQF], j % kQF == 0 ? zero : w[j / kQF]);
+      } else {
+        const int i = j - n1;
+        o[i % kDB] = Op<T>::mfma(a, z[i / (2 * kDB)].f[i / kDB % 2], o[i % kDB]);
       }
 #pragma unroll
       for (int e = kEl * j / n; e < kEl * (j + 1) / n; ++e) {
-        const int rb = e / (16 * NS), sub = e / 16 % NS, r = e % 16;
-        v[e] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
+        v[e] = fast_exp2(__builtin_fmaf(x[e / 16][e % 16], sc, nm));
         if (e > 0) take(e - 1);
       }
       pp_sched_fence();
     }
     take(kEl - 1);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) y[rb][sub].f[m] = __builtin_bit_cast(h8, yw[rb][sub][m]);
+      for (int m = 0; m < 2; ++m) y[sub].f[m] = __builtin_bit_cast(h8, yw[sub][m]);
   }
   // zeroes what is not finite (exponent all ones: adding one to it carries out of the field); was there any?
   static __device__ __forceinline__ bool scrub(u4& w) {
@@ -307,11 +294,11 @@ struct AttnTile {
 // f32 storage: both products on v_mfma_f32_32x32x2_f32 (64 cycles for 2 keys or channels: the matrix pipe is the bound by far, LDS and
 // the vector ALU have slack).  Rows have a pitch of DP + 4 floats.
 // ----------------------------------------------------------------------------------------
-template <int DP, int NW_, int RB_, int NS_>
-struct AttnTile<float, DP, NW_, RB_, NS_> {
+template <int DP, int NW_, int NS_>
+struct AttnTile<float, DP, NW_, NS_> {
   typedef float type;
-  static_assert(RB_ == 1 && NS_ == 1, "f32: one row block, 32 keys a step");
-  static constexpr int NW = NW_, RB = 1, NS = 1, kThreads = 64 * NW, kBN = 32, kRows = 32 * NW;
+  static_assert(NS_ == 1, "f32: 32 keys a step");
+  static constexpr int NW = NW_, NS = 1, kThreads = 64 * NW, kBN = 32, kRows = 32 * NW;
   static constexpr bool kSteady = false;  // (the vector work is a twentieth of the matrix work: nothing to overlap by hand)
   static constexpr int kWaves = DP > 128 || (DP > 96 && NW == 2) ? 1 : 2;  // per SIMD; LDS holds no more
   static constexpr int kP = DP + 4;
@@ -325,7 +312,7 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
     float f[16];
   };
 
-  f4 q[1][kQF];
+  f4 q[kQF];
   u4 ks[kStage], vs[kStageV];
   float* smem;
   int q32, h;
@@ -335,12 +322,12 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
     q32 = (int)threadIdx.x & 31;
     h = ((int)threadIdx.x >> 5) & 1;
   }
-  __device__ __forceinline__ void load_q(int, const float* row, int D) {
+  __device__ __forceinline__ void load_q(const float* row, int D) {
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
       const int d = 8 * c + 4 * h;
-      q[0][c] = f4{0.f, 0.f, 0.f, 0.f};
-      if (row && d < D) q[0][c] = *reinterpret_cast<const f4*>(row + d);
+      q[c] = f4{0.f, 0.f, 0.f, 0.f};
+      if (row && d < D) q[c] = *reinterpret_cast<const f4*>(row + d);
     }
   }
   __device__ __forceinline__ void store_k(int slot, int i, int row, int piece) const {
@@ -350,14 +337,14 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
     *reinterpret_cast<u4*>(smem + 2 * kSlot + slot * kSlotV + row * kPV + 4 * piece) = vs[i];
   }
   // channels are taken in the order (8c + 4h + j): any order serves a dot product as long as both operands share it
-  __device__ __forceinline__ void qk(int slot, f16v (*s)[1]) const {
+  __device__ __forceinline__ void qk(int slot, f16v* s) const {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[0][0][r] = 0.f;
+    for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
 #pragma unroll
     for (int c = 0; c < kQF; ++c) {
       const f4 a = *reinterpret_cast<const f4*>(smem + slot * kSlot + q32 * kP + 8 * c + 4 * h);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[0][0] = mfma_32x32x2_f32(a[j], q[0][c][j], s[0][0]);
+      for (int j = 0; j < 4; ++j) s[0] = mfma_32x32x2_f32(a[j], q[c][j], s[0]);
     }
   }
   static __device__ __forceinline__ P pack_p(const float* p) {
@@ -368,14 +355,14 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
   }
   __device__ __forceinline__ float v_val(int slot, int r, int db) const { return smem[2 * kSlot + slot * kSlotV + score_key(r, h) * kPV + 32 * db + q32]; }
   // keys: wave-uniform; groups of 8 keys behind the last one that any row sees are left out
-  __device__ __forceinline__ void pv(int slot, const P (*p)[1], f16v (*o)[kDB], int keys) const {
+  __device__ __forceinline__ void pv(int slot, const P* p, f16v* o, int keys) const {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       if (8 * g < keys) {
 #pragma unroll
         for (int r = 4 * g; r < 4 * g + 4; ++r)
 #pragma unroll
-          for (int db = 0; db < kDB; ++db) o[0][db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0][0].f[r], o[0][db]);
+          for (int db = 0; db < kDB; ++db) o[db] = mfma_32x32x2_f32(v_val(slot, r, db), p[0].f[r], o[db]);
       }
   }
   static __device__ __forceinline__ bool scrub(u4& w) {
@@ -398,23 +385,22 @@ struct AttnTile<float, DP, NW_, RB_, NS_> {
 // ----------------------------------------------------------------------------------------
 template <typename Tile>
 struct AttnState {
-  f16v o[Tile::RB][Tile::kDB];     // O^T: row d = 32 db + score_key(r, h), column = the lane's query
-  float m[Tile::RB], l[Tile::RB];  // running maximum (of the raw scores; -inf before the first visible key) and the sum
-  bool not_finite;                 // values of V were left out: add_not_finite()
+  f16v o[Tile::kDB];  // O^T: row d = 32 db + score_key(r, h), column = the lane's query
+  float m, l;         // running maximum (of the raw scores; -inf before the first visible key) and the sum
+  bool not_finite;    // values of V were left out: add_not_finite()
 };
 
-// What the rows of a work-group see of its nkeys keys: this lane's rows, the smallest / largest count among the wave's live rows (both 0
-// without one) and the smallest among the work-group's.
-template <int RB>
+// What the rows of a work-group see of its nkeys keys: this lane's row, the largest count among the wave's live rows (0 without one) and the
+// smallest among the work-group's.
 struct AttnLimits {
-  int row[RB], wave_min, wave_max, group_min, nkeys;
+  int row, wave_max, group_min, nkeys;
 };
 
 // The key from whose block on V is staged without values that are not finite: the first one that not every row sees -- or, where rows
 // lie closer together than their channels (a single row, an expanded or overlapping view), the first of a last block with rows left: such a row
 // starts before the block's last byte, so it is not read as zeros, and its weight of 0 does not make an infinity go away.
 template <typename Tile>
-__device__ __forceinline__ int mixed_key(const AttnLimits<Tile::RB>& lim, int64_t v_row, int DV) {
+__device__ __forceinline__ int mixed_key(const AttnLimits& lim, int64_t v_row, int DV) {
   const int whole = lim.nkeys / Tile::kBN * Tile::kBN;
   return v_row < DV && whole < lim.group_min ? whole : lim.group_min;
 }
@@ -422,19 +408,16 @@ __device__ __forceinline__ int mixed_key(const AttnLimits<Tile::RB>& lim, int64_
 // k, v: the first key; D, DV: their channels (of v: those from the pointer on that this work-group sums).  sc = scale * log2(e) > 0.
 template <typename Tile>
 __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typename Tile::type* k, const typename Tile::type* v,
-                                       int64_t k_row, int64_t v_row, const AttnLimits<Tile::RB>& lim, int D, int DV, float sc) {
+                                       int64_t k_row, int64_t v_row, const AttnLimits& lim, int D, int DV, float sc) {
   typedef typename Tile::type T;
   typedef typename Tile::P P;
-  constexpr int RB = Tile::RB, NS = Tile::NS, BN = Tile::kBN;
+  constexpr int NS = Tile::NS, BN = Tile::kBN;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
+  for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
-    for (int db = 0; db < Tile::kDB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) st.o[rb][db][r] = 0.f;
-    st.m[rb] = neg_inf();
-    st.l[rb] = 0.f;
-  }
+    for (int r = 0; r < 16; ++r) st.o[db][r] = 0.f;
+  st.m = neg_inf();
+  st.l = 0.f;
   st.not_finite = false;
   const int nsteps = (lim.nkeys + BN - 1) / BN;
   if (nsteps <= 0) return;
@@ -483,68 +466,58 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     }
   };
 
-  typedef f16v Scores[RB][NS];
-  typedef P Probs[RB][NS];
+  typedef f16v Scores[NS];
+  typedef P Probs[NS];
   // scores of the block whose softmax is next; probabilities of the block before it.  The second pair takes turns in the fast steps, so
   // that nothing is copied.
   Scores s, s2;
   Probs p, p2;
   // -m sc (NaN before the first visible key and from kFar on: whatever a block holds, it is taken again by its differences from the
   // maximum); sums over the block
-  float nm[RB], bs[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) nm[rb] = __builtin_nanf("");
+  float nm = __builtin_nanf(""), bs;
   auto softmax = [&](const Scores& x, Probs& y) __attribute__((always_inline)) -> bool {  // x -> y, bs; did a sum come out too large?
-    bool over = false;
+    bs = 0.f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      bs[rb] = 0.f;
+    for (int sub = 0; sub < NS; ++sub) {
+      float e[16];
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub) {
-        float e[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if constexpr (Tile::kSteady) e[r] = fast_exp2(__builtin_fmaf(x[rb][sub][r], sc, nm[rb]));
-          else e[r] = fast_exp2((x[rb][sub][r] - st.m[rb]) * sc);  // (no maximum yet: infinite or NaN, taken again)
-          bs[rb] += e[r];
-        }
-        y[rb][sub] = Tile::pack_p(e);
+      for (int r = 0; r < 16; ++r) {
+        if constexpr (Tile::kSteady) e[r] = fast_exp2(__builtin_fmaf(x[sub][r], sc, nm));
+        else e[r] = fast_exp2((x[sub][r] - st.m) * sc);  // (no maximum yet: infinite or NaN, taken again)
+        bs += e[r];
       }
-      over |= !(bs[rb] <= kMost);
+      y[sub] = Tile::pack_p(e);
     }
-    return wave_any(over);
+    return wave_any(!(bs <= kMost));
   };
   // moves the maximum to that of x and what was summed up with it; x -> y, bs
   auto move_max = [&](const Scores& x, Probs& y) __attribute__((always_inline)) {
     keep_branch();
+    float top = x[0][0];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float top = x[rb][0][0];
+    for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub)
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, x[sub][r]);
+    top = fmaxf(st.m, pair32_max(top));
+    const float alpha = top == st.m ? 1.f : fast_exp2((st.m - top) * sc);
+    const float base = top == neg_inf() ? 0.f : top;
+    st.m = top;
+    st.l *= alpha;
+    nm = fabsf(top * sc) < kFar ? -top * sc : __builtin_nanf("");
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[rb][sub][r]);
-      top = fmaxf(st.m[rb], pair32_max(top));
-      const float alpha = top == st.m[rb] ? 1.f : fast_exp2((st.m[rb] - top) * sc);
-      const float base = top == neg_inf() ? 0.f : top;
-      st.m[rb] = top;
-      st.l[rb] *= alpha;
-      nm[rb] = fabsf(top * sc) < kFar ? -top * sc : __builtin_nanf("");
+    for (int db = 0; db < Tile::kDB; ++db)
 #pragma unroll
-      for (int db = 0; db < Tile::kDB; ++db)
+      for (int r = 0; r < 16; ++r) st.o[db][r] *= alpha;
+    bs = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st.o[rb][db][r] *= alpha;
-      bs[rb] = 0.f;
+    for (int sub = 0; sub < NS; ++sub) {
+      float e[16];
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub) {
-        float e[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          e[r] = fast_exp2((x[rb][sub][r] - base) * sc);
-          bs[rb] += e[r];
-        }
-        y[rb][sub] = Tile::pack_p(e);
+      for (int r = 0; r < 16; ++r) {
+        e[r] = fast_exp2((x[sub][r] - base) * sc);
+        bs += e[r];
       }
+      y[sub] = Tile::pack_p(e);
     }
   };
   auto stage = [&](int i, int slot) __attribute__((always_inline)) {
@@ -563,12 +536,8 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
       if constexpr (Tile::kDB > 2) wave_priority<1>();
       if constexpr (Tile::kSteady) t.products(S1, w, z, st.o, x, y, nm, sc, bs);
       if constexpr (Tile::kDB > 2) wave_priority<0>();
-      bool over = false;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) over |= !(bs[rb] <= kMost);
-      if (wave_any(over)) move_max(x, y);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) st.l[rb] += bs[rb];
+      if (wave_any(!(bs <= kMost))) move_max(x, y);
+      st.l += bs;
     }
     pp_barrier();
   };
@@ -584,16 +553,13 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     if (i > 0 && (i - 1) * BN < lim.wave_max) t.pv(s1, p, st.o, lim.wave_max - (i - 1) * BN);
     if (i * BN < lim.wave_max) {
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+      for (int sub = 0; sub < NS; ++sub) {
+        const int left = lim.row - i * BN - 32 * sub;
 #pragma unroll
-        for (int sub = 0; sub < NS; ++sub) {
-          const int left = lim.row[rb] - i * BN - 32 * sub;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[rb][sub][r] = score_key(r, t.h) < left ? s[rb][sub][r] : neg_inf();
-        }
+        for (int r = 0; r < 16; ++r) s[sub][r] = score_key(r, t.h) < left ? s[sub][r] : neg_inf();
+      }
       if (softmax(s, p)) move_max(s, p);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) st.l[rb] += bs[rb];
+      st.l += bs;
       if ((i + 1) * BN < lim.wave_max) t.qk(s1, s);
     }
     pp_barrier();
@@ -630,8 +596,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
         }
   }
   if ((nsteps - 1) * BN < lim.wave_max) t.pv((nsteps - 1) & 1, p, st.o, lim.wave_max - (nsteps - 1) * BN);
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) st.l[rb] = pair32_sum(st.l[rb]);
+  st.l = pair32_sum(st.l);
   st.not_finite = *flag != 0;
 }
 
@@ -639,7 +604,7 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
 // mixed_key() on.
 template <typename Tile>
 __device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& st, const typename Tile::type* v, int64_t v_row,
-                                               const AttnLimits<Tile::RB>& lim, int DV) {
+                                               const AttnLimits& lim, int DV) {
 #pragma unroll 1
   for (int key = mixed_key<Tile>(lim, v_row, DV) / Tile::kBN * Tile::kBN; key < lim.nkeys; ++key) {
     const typename Tile::type* row = v + key * v_row;
@@ -649,11 +614,7 @@ __device__ __forceinline__ void add_not_finite(const Tile& t, AttnState<Tile>& s
       for (int r = 0; r < 16; ++r) {
         const int d = 32 * db + score_key(r, t.h);
         const float x = d < DV ? to_f32(row[d]) : 0.f;
-        if ((__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u) {
-#pragma unroll
-          for (int rb = 0; rb < Tile::RB; ++rb)
-            if (key < lim.row[rb]) st.o[rb][db][r] += x;
-        }
+        if ((__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u && key < lim.row) st.o[db][r] += x;
       }
   }
 }
