@@ -48,7 +48,7 @@ __device__ __forceinline__ void store_part(const PartsK& a, const Tile& t, const
 }
 
 // A row's D values are DL threads of 4, and PG groups of such threads take every PG-th part each, four parts' loads in flight; then the groups'
-// results are joined in LDS.  (One thread per 4 values walking all parts took 17 us for 33 parts of 1024 rows of 128, this takes 5.)
+// results are joined in LDS.  (One thread per 4 values walking all parts: 31 us for 32 tokens behind 8192 keys in all, this 26.)
 template <typename Tile, int DL>
 __global__ void __launch_bounds__(256) attention_join_kernel(const PartsK a, int pg_log2) {
   typedef typename Tile::type T;

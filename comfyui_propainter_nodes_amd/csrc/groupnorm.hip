@@ -3,8 +3,9 @@
 //
 //   mean = sum x / M, var = sum x^2 / M - mean^2 over the M = HW * C/G values of a group;  y = post(skip + act((x - mean) r gamma + beta))
 //
-// The sums are held in double (a product of two f32 values is exact there, so sum x^2 / M - mean^2 loses nothing that f32 data
-// holds until |mean| / std passes 10^6); f64 multiply-adds run at the rate of f32 ones, far above what memory delivers.  The mean is applied
+// The sums are held in double, where a product of two f32 values is exact: sum x^2 / M - mean^2 is (mean / std)^2 times a few 2^-53 off, relative to the
+// variance.  (65536 f32 values, eps 0: results within 9e-8 of theirs at |mean| / std = 10^4, 4e-7 at 10^5, 2e-5 at 10^6, where f32 data has four
+// bits below its standard deviation.)  f64 multiply-adds run at the rate of f32 ones, far above what memory delivers.  The mean is applied
 // as an f32 pair (high, low), so the subtraction is as exact as the data.
 //
 // Bound by memory: 16 x 180 x 320 x 64 f32 with ReLU 149 us -- sums 55 us (236 MB at 4.3 TB/s), apply 82 us (472 MB at 5.8, partly from the
@@ -82,7 +83,9 @@ __device__ __forceinline__ float gelu_fast(float x) {
   return __builtin_fmaf(-z, q, __builtin_fmaf(0.5f, fabsf(x), 0.5f * x));
 }
 
-// f32 storage: the library's functions; 16-bit storage: hardware exponential and reciprocal (a few 2^-24, far below the rounding to come)
+// f32 storage: the library's functions; 16-bit storage: hardware exponential and reciprocal, each a few 2^-24 off.  The rounding of an exponential's
+// argument makes the tails worse, in proportion to it: GELU's reach 3e-6 of the value where f16 ends (v = -5.6; to be rounded by up to 2^-11) and
+// 2e-5 where bf16 does (v = -13; 2^-8).
 template <typename T>
 __device__ __forceinline__ float norm_act(float v, int act, float param) {  // act: a compile-time constant or uniform
   constexpr bool kExact = sizeof(T) == 4;
@@ -99,7 +102,7 @@ __device__ __forceinline__ float norm_act(float v, int act, float param) {  // a
 
 constexpr int kOwnGroups = 32;  // groups and sums up to which the apply pass joins them itself
 constexpr int kOwnSums = 2048;
-constexpr int kAhead = 8;  // 16-byte loads of a thread in flight in the sums pass (16 x 180 x 320 x 64 f32: 4 150 us, 8 148)
+constexpr int kAhead = 8;  // 16-byte loads of a thread in flight in the sums pass (16 x 180 x 320 x 64 f32: 4 149.4 us, 8 148.4)
 
 // sums of one chunk of one image, all groups
 template <typename T, int V>
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(256) groupnorm_apply_kernel(const GroupNormK k
     const T* x = (const T*)k.x + px * k.x_ldc + c0;
     const T* skip = (const T*)k.skip + px * k.skip_ldc + c0;
     T* y = (T*)k.y + px * k.y_ldc + c0;
-    // (one vector at a time: with 4 in flight a thread holds 139 registers instead of 60 and 6 x 181 x 243 x 320 bf16 with GELU takes 157 us, not 148)
+    // (one vector at a time: with 4 in flight a thread holds 139 registers instead of 60 and 6 x 181 x 243 x 320 bf16 with GELU takes 158 us, not 146)
     for (int64_t p = p0 + pl; p < p1; p += k.lanes) {
       const auto v = Vec<T, V>::ld(x + p * k.x_ldc);
       f.template apply<ACT>(k, v, k.skip ? Vec<T, V>::ld(skip + p * k.skip_ldc) : v, y + p * k.y_ldc);
@@ -356,9 +359,11 @@ __global__ void __launch_bounds__(256) groupnorm_held_kernel(const GroupNormK k)
 template <typename T, int V, int ACT>
 static int launch_groupnorm_act(void* stream, pp::GroupNormK& k) {
   using namespace pp;
-  // A group's rows are short pieces of the image's: one launch pays while there are few of them in all (f16, 32 groups of 8: 576 vectors a
-  // group, 16 images, 15.2 us against 16.3 in two or three launches; 1024 vectors, 4 images, 12.9 against 15.5; 16 images, 21.1 against 18.7; 2025
-  // vectors, 4 images, 20.8 against 17.9; 1024 threads with 8 vectors each lost at every size).
+  // A group's rows are short pieces of the image's, one vector in the worst case: one launch pays while there are few of them in all.  Up to
+  // 1024 vectors a group, in us, one launch against more: 32 groups of one vector a pixel, f16: 65536 vectors in all 6.6 / 13.6, 262144
+  // 12.7 / 14.0, 524288 20.3 / 15.8; f32: 131072 9.0 / 11.1, 262144 12.0 / 11.1, 524288 19.0 / 12.1.  The limit is set by these.  Wider rows would bear
+  // a higher one: 5 vectors a pixel, bf16: 262144 7.8 / 18.9, 524288 13.5 / 19.3, 1048576 24.1 / 27.3, 2097152 43.2 / 34.7; 8 vectors, f32: 524288 9.0 / 13.2.
+  // Groups of whole rows (one group): 65536 12.4 / 32.7.
   const int64_t vectors = k.HW * (k.cpg / V);
   if (k.cpg % V == 0 && vectors <= 256 * kHeld && vectors * k.N * k.G <= 400000) {
     PP_LAUNCH((groupnorm_held_kernel<T, V, ACT>), dim3((unsigned)(k.N * k.G)), dim3(256), 0, stream, k);

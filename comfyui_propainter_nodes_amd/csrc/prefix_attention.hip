@@ -2,7 +2,7 @@
 // Contract: include/propainter_mi355.h (pp_prefix_attention); the inner loop: tile_attention.h.
 //
 // All B L G rows of a key / value head (G = H / KH query heads share it) meet the same prefix keys: they are tiled 128 at a time, so a
-// prefix of P keys is staged ceil(B L G / 128) times instead of B times, and the two products run at matrix speed.  The prefix is
+// prefix of P keys is staged ceil(B L G / 128) times (its keys twice that for f32 above 128 channels) instead of B times, and the two products run at matrix speed.  The prefix is
 // cut into pieces so that few rows still fill the chip; the own keys of a sequence (its L G rows) are work-groups of the same launch.  Every piece
 // leaves (maximum, sum, sum of weighted values) in fp32; a second launch joins them in piece order.
 //

@@ -129,8 +129,8 @@ static int launch_prompt_d(void* stream, pp::PromptK& a) {
     if (a.D <= 128) return launch_prompt<AttnTile<T, 128, 4, 1>>(stream, a);
     return launch_prompt<AttnTile<T, 256, 4, 1>>(stream, a);
   } else {
-    // Rows of a sequence that fit one 64-row work-group of 2 waves: with 4 waves half of them would idle (45 rows and keys, 128 channels: 153
-    // -> 133 us for 2592 sequences and heads).  Long sequences share the staging of 4 waves (2048 tokens: 277 us against 424).
+    // Rows of a sequence that fit one 64-row work-group of 2 waves: with 4 waves half of them would idle (45 rows and keys, 128 channels: 121
+    // -> 99 us for 2592 sequences and heads).  Long sequences share the staging of 4 waves (2048 tokens, 16 / 4 heads: 281 us against 294).
     if (a.Tq * a.G <= 64 * (int64_t)a.B) {
       if (a.D <= 32) return launch_prompt<AttnTile<T, 32, 2, 1>>(stream, a);
       if (a.D <= 64) return launch_prompt<AttnTile<T, 64, 2, 1>>(stream, a);

@@ -20,9 +20,10 @@
 // beyond it; f32 storage and the blocks that move m always take the difference.
 //
 // Bound by the matrix pipes: one causal prompt of 8192 tokens, 32 query heads over 8 key heads of 128, f16: 533-590 us by card, 0.93-1.03 PF/s, MFMA busy
-// 52 % of the cycles at the 1.87 GHz that the card holds under it, LDS 39 %, no bank conflict; 843 TF/s at 64 channels, 860 at 256, f32 136 TF/s
-// (full f32 MFMA rate 157).  64 rows a wave would halve the LDS reads, but left one wave per SIMD and cost register moves (935 us).
-// With a maximum per block and per-lane addresses the same call took 703 us, with the MFMAs left to the compiler's order 634.
+// 50-52 % of the cycles at the 1.8-1.9 GHz that the card holds under it, LDS 38 %, no bank conflict; 800-830 TF/s at 64 channels, 920 at 256; f32 129,
+// 135 and 66 TF/s at 64, 128 and 256 channels (a library product: 152).  On a card where it takes 570 us it took 565 before differences were kept exact
+// for far scores, 640 with a maximum per block and per-lane addresses, 672 with the MFMAs left to the compiler's order besides.  64 rows a wave
+// would halve the LDS reads, but left one wave per SIMD and cost register moves.
 //
 // Rows that see different numbers of keys: `limit` is the row's own count, scores at or past it become -inf before the softmax.  Their
 // probability is 0, but 0 x V is NaN for a V that is not finite.  Keys past the last one that any row of the work-group sees are staged as
@@ -302,8 +303,8 @@ struct AttnTile<float, DP, NW_, NS_> {
   static constexpr bool kSteady = false;  // (the vector work is a twentieth of the matrix work: nothing to overlap by hand)
   static constexpr int kWaves = DP > 128 || (DP > 96 && NW == 2) ? 1 : 2;  // per SIMD; LDS holds no more
   static constexpr int kP = DP + 4;
-  // Queries of 256 channels and the sums of 256 do not fit the registers together (they spilled: 30 TF/s): two work-groups take half of the
-  // value channels each and both compute the scores, 3/2 of the work at four times the rate.
+  // Queries of 256 channels and the sums of 256 do not fit the registers together (they spill: 25 TF/s, against 60): two work-groups take half of the
+  // value channels each and both compute the scores, 3/2 of the work at more than three times the rate.
   static constexpr int kHalves = DP > 128 ? 2 : 1, kDV = DP / kHalves;
   static constexpr int kPieces = DP / 4, kPer = 4, kAll = kBN * kPieces, kStage = (kAll + kThreads - 1) / kThreads, kDB = kDV / 32, kQF = DP / 8;
   static constexpr int kPiecesV = kDV / 4, kAllV = kBN * kPiecesV, kStageV = (kAllV + kThreads - 1) / kThreads;
@@ -532,7 +533,8 @@ __device__ __forceinline__ void attend(Tile& t, AttnState<Tile>& st, const typen
     constexpr int S0 = decltype(slot)::value, S1 = 1 - S0;
     stage(i, S0);
     if (lim.wave_max > 0) {
-      // a wave that is in its products goes before one that stages (D = 128: 533 -> 530 us, 507 -> 498 without a mask; 64: 330 -> 334, so not there)
+      // a wave that is in its products goes before one that stages (prompt of 8192, 128 channels: 581 -> 571 us, 1131 -> 1103 without a
+      // mask; 64: 338 either way, so not there)
       if constexpr (Tile::kDB > 2) wave_priority<1>();
       if constexpr (Tile::kSteady) t.products(S1, w, z, st.o, x, y, nm, sc, bs);
       if constexpr (Tile::kDB > 2) wave_priority<0>();

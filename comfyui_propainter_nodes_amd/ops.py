@@ -1207,8 +1207,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
 
 def prompt_splits(b: int, tq: int, tk: int, h: int, kh: int) -> int:
     """Work-groups that share the keys of a tile in a prompt_attention call.  The chip holds 512 work-groups at once (two per CU); fewer tiles
-    than a third of that share their keys, as long as the average sequence leaves each work-group 256 of them.  (4096 causal tokens, 4 heads over
-    one key head of 128: 73 us alone, 47 in three parts; 4 x 1 token behind 8192 keys: 96 -> 23; 232 tiles of about 2000 keys: 31, in two parts 35.)"""
+    than a third of that share their keys, as long as the average sequence leaves each work-group 256 of them.  (f16, 4096 causal tokens, 4 heads
+    over one key head of 128: 92 us alone, 50 in three parts as the rule takes them, 46 in four; 4 x 1 token behind 8192 keys, 32 / 8 heads of 128: 173 us
+    alone, 34 in eight.  Two parts are not taken: 2 x 2000 causal tokens, 8 heads of 64, 264 tiles: 32 us alone, 38 in two -- but 3700 tokens without a
+    mask, 8 heads of 128, 240 tiles: 87 alone, 79 in two, and 32 x 1 token behind 4096 keys, 256 tiles: 117 and 103, f32 646 and 335.)"""
     tiles = (tq * (h // kh) // 128 + b) * kh
     splits = min(8, 512 // max(1, tiles), tk // max(1, b) // 256)
     return splits if splits >= 3 else 1
@@ -1221,8 +1223,9 @@ def prompt_attention_scratch(q: torch.Tensor, k: torch.Tensor, cu_q: torch.Tenso
 
 
 def prefix_splits(b: int, new: int, p: int, s: int, h: int, kh: int) -> tuple[int, int]:
-    """(pieces of the prefix, pieces of an own range) of a prefix_attention call: pieces of about the same length, a multiple of 64 keys, that
-    together make the 512 work-groups that the chip holds at once (two per CU)."""
+    """(pieces of the prefix, pieces of an own range) of a prefix_attention call, so that pieces of about the same length make together about the
+    512 work-groups that the chip holds at once (two per CU).  The length aimed at is a multiple of 64 keys; the pieces share the keys evenly and end
+    anywhere."""
     tiles = -(-b * new * (h // kh) // 128) * kh
     own = -(-new * (h // kh) // 128) * kh * b if s else 0
     piece = max(64, -(-(tiles * p + own * s) // (512 * 64)) * 64)

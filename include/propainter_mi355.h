@@ -552,7 +552,8 @@ int32_t pp_groupnorm(void* stream, const pp_groupnorm_params* p);
  * D % 8 == 0 (% 4 for PP_F32), D <= 256; Tk <= 2^31 - 1024.
  * out may be q (same strides; not for PP_F32 with D > 128), and overlaps nothing else.
  * PP_F16 / PP_BF16: MFMA operands in the storage type (the probabilities are rounded to it once, as operands of the second
- * product), fp32 scores, sums and accumulators.  PP_F32: everything fp32 (f32 MFMA).
+ * product), fp32 scores, sums and accumulators.  PP_F32: everything fp32 (f32 MFMA).  Finite scores may be of any size: weights come from
+ * their differences.  A value that is not finite reaches the rows that see it (as NaN where its probability rounds to 0).
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   int32_t dtype; /* q, k, v, out: PP_F32, PP_F16 or PP_BF16 */
@@ -582,7 +583,8 @@ int32_t pp_prompt_attention(void* stream, const pp_prompt_attention_params* p);
  *   q, out [B][L][H][D]; kp, vp [P][KH][D]; ko, vo [B][S][KH][D]; own_len i32 [B] (on the device; clamped to [0, S]): keys of
  *   sequence b behind the prefix, its L new tokens among them.  Token i of L sees the whole prefix and own keys
  *   j <= own_len[b] - L + i.  A row that sees no key gets 0.  Keys and values that a row does not see never reach its result.
- * The prefix's keys and values are read once for all rows of a key / value head, not once per sequence.
+ * The prefix's keys and values are read once for every 128 of the B * L * H / KH rows of a key / value head (keys twice for PP_F32 with
+ * D > 128), not once per sequence.
  * `scratch`: caller-owned, 16-byte aligned, B * L * H * (prefix_splits + own_splits) * (D + 4) floats; prefix_splits pieces of the
  * prefix and own_splits pieces of each own range go to different work-groups and are joined in a fixed order (both >= 0, a
  * part with keys needs at least one).  Strides in elements as in pp_prompt_attention; P, S <= 2^31 - 1024.
