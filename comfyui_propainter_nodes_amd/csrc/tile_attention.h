@@ -6,6 +6,9 @@
 //   online softmax    lane-local, one exchange between lanes l and l ^ 32; fp32 maxima, sums and accumulators
 //   O^T += V^T . P^T  the lane's own probabilities are the B operand, V^T fragments come out of LDS transposed (f16 / bf16:
 //                     ds_read_b64_tr_b16; f32: one value per lane)
+// A 16-bit product takes 16-bit operands: a probability is rounded to the storage type once, half a step of its own size, before it meets V (its f32
+// value goes into the sum).  The error against 64 bits is 1.1 to 1.4 times that of f32 probabilities with the result rounded once (f16 2.5e-4 against
+// 1.9e-4 on the long prompt, bf16 2.3e-3 against 1.7e-3 behind a prefix); f32 operands would run at a seventh of the rate.
 // Step i works on three key blocks at once -- the softmax of block i, the second product of block i - 1 and the first of block i + 1 -- so
 // every MFMA of a step is independent of its exponentials.  K and V pass through two LDS slots each; their loads are issued a step
 // before they are stored, one barrier a step.
